@@ -22,6 +22,11 @@ FLAGS = [
     # forms on its own need register shuffles -- and, in streaming loops, copies of loads still in flight -- that cost
     # blend_bwd 5 % and exposed a memory round trip per row in photometric_bwd (DESIGN s3, round 3)
     "-fno-slp-vectorize",
+    # no packed fp32 instructions: some of their forms have given wrong results now and then on this hardware, in ways a
+    # test does not reliably show.  A float2v fma becomes two plain ones with the same rounding; a 1280x1024 / 300 000-Gaussian
+    # mapping step takes 0.580 ms either way (blend_fwd 106.7 -> 104.6 us, blend_bwd 226 -> 229 us).  (hipcc's host pass
+    # prints that it does not know the feature.)
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
 # FSGS_DIAG=1: the diagnostics flavour -- the hooks of csrc/raster_kernels.h (diag_env: per-tile stamps, injected dispatch
 # orders, lane-utilisation counters) and the experiment switches (FSGS_EXP_*, honoured ONLY together with the hooks).  A
@@ -81,8 +86,9 @@ def _compile(src):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("hipcc failed for %s:\n%s\n%s" % (src, r.stdout, r.stderr))
-        if r.stderr.strip():
-            sys.stderr.write(r.stderr)
+        told = [ln for ln in r.stderr.splitlines() if "-packed-fp32-ops" not in ln]
+        if any(ln.strip() for ln in told):
+            sys.stderr.write("\n".join(told) + "\n")
         with open(stamp, "w") as f:
             f.write(want)
     return obj

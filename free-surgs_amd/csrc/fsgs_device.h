@@ -12,7 +12,7 @@
 
 namespace fsgs {
 
-typedef float float2v __attribute__((ext_vector_type(2)));  // a register pair: elementwise fma on it is one v_pk_fma_f32
+typedef float float2v __attribute__((ext_vector_type(2)));  // a register pair with elementwise arithmetic (two plain instructions)
 
 // ---- scalar broadcast of one lane's value (v_readlane_b32: the index must be wave-uniform) ----
 __device__ __forceinline__ float readlane(float v, int lane) {

@@ -89,7 +89,7 @@ __device__ __forceinline__ void photometric_fwd_tile(const int tile_id, int C, i
                                                      const float *__restrict__ presence, float *__restrict__ maps,
                                                      float *__restrict__ partials) {
   // image and target of a pixel side by side, the moments as two pairs: one 8-byte LDS access moves a pair and the 11-tap
-  // filters of a pair are one v_pk_fma_f32 per tap, each component still accumulating its taps in the order k = 0..10.
+  // filters of a pair are one elementwise fma per tap (two plain instructions), each component still accumulating its taps in the order k = 0..10.
   // SSIM needs the two second moments e11 = G*x^2 and e22 = G*y^2 only as their SUM (sigma1^2 + sigma2^2 =
   // e11 + e22 - m1^2 - m2^2, utils/loss_utils.py:76-81), so FOUR filters are run, not five: (m1, m2) and (e11 + e22, e12).
   // That is a fifth of the filter work and, more to the point, 36.6 KB of LDS instead of 42.2: four workgroups per CU instead

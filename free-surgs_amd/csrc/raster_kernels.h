@@ -979,7 +979,7 @@ __global__ __launch_bounds__(64) void blend_fwd_kernel(
   // T[k] > 0: transmittance of a pixel that is still blending; a FINISHED pixel (T (1 - alpha) < 1e-4 seen, or outside
   // the image) keeps its transmittance with the sign flipped -- the "done" flag costs no register and one compare
   // (86 -> 80 VGPRs: six waves per SIMD; one VALU less per quadrant body)
-  // the colour sums are kept as channel PAIRS: a pair's update is one v_pk_fma_f32 with the record's (x, y) / (z, w) halves
+  // the colour sums are kept as channel PAIRS: a pair's update is one elementwise fma with the record's (x, y) / (z, w) halves
   // as they come out of the broadcast read.  Written out here because the build runs without the SLP vectoriser (which
   // formed these pairs by itself, but cost blend_bwd 5 % with the register shuffles it added there).
   constexpr int CP = (C + 1) / 2;
