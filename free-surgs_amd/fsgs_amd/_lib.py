@@ -80,6 +80,18 @@ class FsgsAdamGroup(C.Structure):
                 ("n", C.c_int64), ("lr", C.c_float), ("step", C.c_int32)]
 
 
+# FsgsAdamWTensor / FsgsAdamWMoments / FsgsGradTensor are rows of 64-bit words (include/fsgs.h): the optimiser fills them as flat
+# array('q') buffers, several times faster than ctypes fields over hundreds of tensors
+ADAMW_TENSOR_WORDS, ADAMW_MOMENTS_WORDS, GRAD_TENSOR_WORDS = 8, 6, 3
+ADAMW_BLOCK = 128
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+
+
+class FsgsAdamWHyper(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double), ("eps", C.c_double),
+                ("weight_decay", C.c_double), ("step", C.c_int64), ("step_dev", C.c_void_p), ("lr_dev", C.c_void_p)]
+
+
 class FsgsError(RuntimeError):
     def __init__(self, code, where, detail=""):
         self.code = code
@@ -185,6 +197,12 @@ _PROTOTYPES = {
                                  C.c_double, C.c_double, C.c_double, _vp, _vp]),
     "fsgs_pose_frame_begin": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "fsgs_adam_step": (_i, [_i, C.POINTER(FsgsAdamGroup), C.c_double, C.c_double, C.c_double, _vp]),
+    "fsgs_adamw_scratch_bytes": (_sz, [_i]),
+    "fsgs_adamw_step": (_i, [_i, _vp, _i, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "fsgs_adamw_moments": (_i, [_i, _vp, _i, _i, _vp]),
+    "fsgs_grad_norm_scratch_bytes": (_sz, [_i]),
+    "fsgs_grad_norm": (_i, [_i, _vp, C.c_float, _vp, _sz, _vp, _vp]),
+    "fsgs_grad_scale": (_i, [_i, _vp, _vp, _vp]),
     "fsgs_densify_plan": (_i, [_i, _vp, _vp, _vp, _vp, C.c_float, C.c_float, C.c_float, C.c_float, _i, _vp, _vp]),
     "fsgs_densify_apply": (_i, [_i, _vp, _vp, C.POINTER(C.c_int32), _i, C.POINTER(FsgsDensifyGroup), _vp, _vp, _vp,
                                 _vp]),

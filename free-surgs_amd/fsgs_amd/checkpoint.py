@@ -28,6 +28,12 @@ def portable_state_dict(optimizer):
     """optimizer.state_dict() as torch.optim.Adam would have written it: every `step` a 0-d float32 CPU tensor and
     every param_group carrying the keys torch's Adam reads (FusedAdam's own defaults are lr / betas / eps only)."""
     sd = optimizer.state_dict()
+    if hasattr(optimizer, "widen"):  # FusedAdamW: moments as values whatever their width, in entries of their own
+        for packed, group in zip(sd["param_groups"], optimizer.param_groups):
+            packed["decoupled_weight_decay"] = True
+            for i, p in zip(packed["params"], group["params"]):
+                if i in sd["state"]:
+                    sd["state"][i] = optimizer.wide_state(p)
     for st in sd["state"].values():
         if "step" in st and not torch.is_tensor(st["step"]):
             st["step"] = torch.tensor(float(st["step"]), dtype=torch.float32)
@@ -69,7 +75,7 @@ def restore_gaussians(pc, model_args, opt=OptimizationParams, eps=1e-15, fused=T
     pc.variables["xyz_gradient_accum"] = torch.zeros_like(plain(model_args[8]))
     pc.variables["denom"] = torch.zeros_like(plain(model_args[9]))
     pc.spatial_lr_scale = float(model_args[11])
-    pc.training_setup(opt, eps=eps, fused=fused)
+    pc.training_setup(opt, eps=eps, fused=fused, adamw=pc.adamw)
     sd = model_args[10]
     pc.optimizer.load_state_dict({
         "param_groups": sd["param_groups"],

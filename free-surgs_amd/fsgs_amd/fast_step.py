@@ -551,6 +551,8 @@ class FastStepper:
             b = self._buffers(pc.num_points, H, W, n_patches, dev)
             stream = _lib.current_stream()
             fused_ok = step_optimizer and grad_sync is None and isinstance(pc.optimizer, optim.FusedAdam)
+            if reduce_compact is not None and isinstance(pc.optimizer, optim.FusedAdamW):
+                raise RuntimeError("reduce_compact feeds optim.FusedAdam; with optim.FusedAdamW reduce the gradients with grad_sync")
             # single view, single rank: the backward feeds Adam directly (no gradient tensors at all)
             fuse_adam = self.fuse_adam and fused_ok and len(timesteps) == 1 and reduce_compact is None
             if fuse_adam:

@@ -49,6 +49,7 @@ class GaussianCloud:
         self.variables = {"max_radii2D": z(P), "xyz_gradient_accum": z(P, 1), "denom": z(P, 1),
                           "scene_radius": torch.tensor(float(scene_radius), device=device)}
         self.optimizer = None
+        self.adamw = None  # options of optim.FusedAdamW, or None: optim.FusedAdam
         self.cam = None
 
     @property
@@ -80,14 +81,22 @@ class GaussianCloud:
         if self.active_sh_degree < self.max_sh_degree:
             self.active_sh_degree += 1
 
-    def training_setup(self, opt=OptimizationParams, eps=1e-15, fused=True):
+    def training_setup(self, opt=OptimizationParams, eps=1e-15, fused=True, adamw=None):
         """Adam with the reference's per-group learning rates (scene/gaussian_model.py:382-409).
-        fused=True: one HIP launch per step (fsgs_amd.optim.FusedAdam); False: torch.optim.Adam."""
+        fused=True: one HIP launch per step (fsgs_amd.optim.FusedAdam); False: torch.optim.Adam.
+        adamw: a dict of options for fsgs_amd.optim.FusedAdamW instead (weight_decay -- 0 unless given --, state_bits=8,
+        max_grad_norm, betas, ...), kept for the optimizers that initialize_optimizer and a restored checkpoint build;
+        {} is Adam's arithmetic with FusedAdamW's state.  The step driver then runs its unfused optimizer step."""
+        self.adamw = None if adamw is None else dict(adamw)
         lr = {"_xyz": opt.position_lr_init * self.spatial_lr_scale, "_features_dc": opt.feature_lr,
               "_features_rest": opt.feature_lr / 20.0, "_opacity": opt.opacity_lr, "_scaling": opt.scaling_lr,
               "_rotation": opt.rotation_lr}
         groups = [{"params": [self.params[k]], "lr": lr[k], "name": k} for k in PARAM_NAMES]
-        if fused:
+        if self.adamw is not None:
+            from .optim import FusedAdamW
+
+            self.optimizer = FusedAdamW(groups, **{"lr": 0.0, "eps": eps, "weight_decay": 0.0, **self.adamw})
+        elif fused:
             from .optim import FusedAdam
 
             self.optimizer = FusedAdam(groups, lr=0.0, eps=eps)
@@ -115,6 +124,7 @@ class GaussianCloud:
     def _swap_params(self, new_tensors, moment_fn):
         """Install new leaf tensors for every group and transform the Adam moments with
         moment_fn(name, old_moment) -> new_moment (the reference's state surgery, :501-580)."""
+        self._widen_moments()
         for group in self.optimizer.param_groups:
             name = group["name"]
             old = group["params"][0]
@@ -126,6 +136,13 @@ class GaussianCloud:
                 self.optimizer.state[new] = state
             group["params"][0] = new
             self.params[name] = new
+
+    def _widen_moments(self):
+        """8-bit Adam moments (blocks that span rows) as fp32 ones in front of a row operation; the optimizer's next step
+        brings them back to 8 bits"""
+        for group in self.optimizer.param_groups:
+            if group.get("state_bits") == 8:
+                self.optimizer.widen(group["params"][0])
 
     def prune_points(self, mask):
         keep = ~mask
@@ -205,6 +222,8 @@ class GaussianCloud:
         acc = self.variables["xyz_gradient_accum"].detach().reshape(-1).contiguous().float()
         den = self.variables["denom"].detach().reshape(-1).contiguous().float()
         counts = torch.empty((4, P), dtype=torch.int32, device=dev)
+        if self.optimizer is not None:
+            self._widen_moments()
         with torch.cuda.device(dev):
             stream = _lib.current_stream()
             _lib.check(lib.fsgs_densify_plan(P, _lib.ptr(acc), _lib.ptr(den), _lib.ptr(self.params["_scaling"].detach()),
@@ -261,6 +280,8 @@ class GaussianCloud:
             if group["name"] != "_opacity":
                 continue
             old = group["params"][0]
+            if group.get("state_bits") == 8:
+                self.optimizer.widen(old)
             state = self.optimizer.state.pop(old, None)
             t = new.detach().contiguous().requires_grad_(True)
             if state is not None and "exp_avg" in state:
@@ -276,7 +297,11 @@ class GaussianCloud:
               "_features_rest": self.opt.feature_lr / 20.0, "_opacity": self.opt.opacity_lr,
               "_scaling": self.opt.scaling_lr, "_rotation": self.opt.rotation_lr}
         groups = [{"params": [self.params[k]], "lr": lr[k], "name": k} for k in PARAM_NAMES]
-        if fused:
+        if self.adamw is not None:
+            from .optim import FusedAdamW
+
+            self.optimizer = FusedAdamW(groups, **{"weight_decay": 0.0, **self.adamw})
+        elif fused:
             from .optim import FusedAdam
 
             self.optimizer = FusedAdam(groups)

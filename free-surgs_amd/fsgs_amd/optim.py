@@ -1,7 +1,9 @@
 """Fused optimiser pieces: `FusedAdam` (drop-in for the torch.optim.Adam instances the reference
 builds at scene/gaussian_model.py:372-378,408 and scene/pose_optimizer.py:489-493 -- same param_groups
-and state layout, so densification's state surgery keeps working) and the densification statistics."""
+and state layout, so densification's state surgery keeps working), `FusedAdamW` (decoupled weight decay, any number of
+tensors, 16-bit parameters, moments in 32 or 8 bits), `grad_norm` / `clip_grad_norm_`, and the densification statistics."""
 import ctypes as C
+from array import array
 
 import torch
 
@@ -54,6 +56,442 @@ class FusedAdam(torch.optim.Optimizer):
                     _lib.check(lib.fsgs_adam_step(len(chunk), arr, b1, b2, eps, stream), "fsgs_adam_step")
                 mark_updated([it[0] for it in items])
         return None
+
+
+_DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
+_F32, _Q = torch.float32, torch.float8_e4m3fn
+
+
+def _dense(t):
+    """every element of t's span of memory belongs to t exactly once (contiguous up to the order of the dimensions)"""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda ns: ns[1]):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _same_layout(a, b):
+    return a.shape == b.shape and ((a.is_contiguous() and b.is_contiguous()) or a.stride() == b.stride())
+
+
+def _address(buf):
+    return buf.buffer_info()[0]
+
+
+class _on:
+    """the device of a bucket of tensors made current (nothing to do where it is already)"""
+
+    def __init__(self, device):
+        self.guard = torch.cuda.device(device) if device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _check_grad(g, name="gradient"):
+    if g.layout != torch.strided:
+        raise RuntimeError("%s: sparse gradients are not supported" % name)
+    if not g.is_cuda:
+        raise RuntimeError("%s: needs CUDA/HIP tensors; there is no CPU fallback" % name)
+    if g.dtype not in _DTYPES:
+        raise TypeError("%s: float32, bfloat16 or float16, got %s" % (name, g.dtype))
+
+
+def _norm_of(lib, grads, max_norm):
+    """(float32 [2] = {norm, factor}) of gradients on one device, on the current stream of that device"""
+    dev = grads[0].device
+    table, keep = array("q"), []
+    for g in grads:
+        if not _dense(g):
+            g = g.contiguous()
+            keep.append(g)
+        table.extend((g.data_ptr(), g.numel(), _DTYPES[g.dtype]))
+    n = len(grads)
+    nbytes = lib.fsgs_grad_norm_scratch_bytes(n)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    out = torch.empty(2, dtype=_F32, device=dev)
+    _lib.check(lib.fsgs_grad_norm(n, _address(table), float(max_norm), scratch.data_ptr(), nbytes, out.data_ptr(),
+                                  _lib.current_stream()), "fsgs_grad_norm")
+    return out
+
+
+def _one_device(grads, who):
+    dev = grads[0].device
+    for g in grads:
+        _check_grad(g, who)
+        if g.device != dev:
+            raise RuntimeError("%s: gradients on %s and on %s; call it once for each device" % (who, dev, g.device))
+    return dev
+
+
+def _max_norm(v):
+    v = float(v)
+    if not v >= 0.0:
+        raise ValueError("max_norm is a number that is not negative, got %r" % v)
+    return v
+
+
+@torch.no_grad()
+def grad_norm(tensors):
+    """Global 2-norm of any number of float32 / bfloat16 / float16 tensors on one device: a 0-d float32 tensor there, no host
+    synchronisation.  Squares are summed in 64 bits and in a fixed order."""
+    tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    lib = _lib.load()
+    with _on(_one_device(tensors, "grad_norm")):
+        return _norm_of(lib, tensors, float("inf"))[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """torch.nn.utils.clip_grad_norm_ in three launches per 48 tensors: the gradients' global 2-norm, and every gradient
+    scaled in place by min(1, max_norm / (norm + 1e-6)); where that factor is 1 no gradient is read again.  Returns the norm
+    (0-d float32) without a host synchronisation, unless error_if_nonfinite asks for one."""
+    if float(norm_type) != 2.0:
+        raise ValueError("clip_grad_norm_: the 2-norm only, got norm_type=%r" % (norm_type,))
+    max_norm = _max_norm(max_norm)
+    parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.tensor(0.0)
+    if len({id(g) for g in grads}) != len(grads):
+        raise ValueError("clip_grad_norm_: a parameter is given twice")
+    lib = _lib.load()
+    dev = _one_device(grads, "clip_grad_norm_")
+    table, strided = array("q"), []
+    for g in grads:
+        if _dense(g):
+            table.extend((g.data_ptr(), g.numel(), _DTYPES[g.dtype]))
+        else:
+            strided.append(g)
+    with _on(dev):
+        out = _norm_of(lib, grads, max_norm)
+        norm, coef = out[0], out[1]
+        if error_if_nonfinite and not bool(torch.isfinite(norm)):
+            raise RuntimeError("clip_grad_norm_: the gradients' norm is %s" % float(norm))
+        rc = lib.fsgs_grad_scale(len(table) // _lib.GRAD_TENSOR_WORDS, _address(table), coef.data_ptr(), _lib.current_stream())
+        if rc == _lib.FSGS_ERR_INVALID:
+            raise ValueError("clip_grad_norm_: two of the gradients share memory")
+        _lib.check(rc, "fsgs_grad_scale")
+        for g in strided:  # slices of other tensors; expanded ones torch itself refuses to write
+            g.copy_(g.float() * coef)
+        mark_updated(grads)
+    return norm
+
+
+class FusedAdamW(torch.optim.Optimizer):
+    """torch.optim.AdamW semantics (decoupled weight decay; no amsgrad) over any number of tensors, 48 a kernel launch.
+
+    Parameters may be float32, bfloat16 or float16 (gradients of the same type), dense in memory, on one or several devices.
+    Options, each also per param_group except max_grad_norm:
+
+    state_bits      32: state[p] = {'step', 'exp_avg', 'exp_avg_sq'} in float32, whatever the parameter's type.
+                    8: {'step', 'exp_avg_q', 'exp_avg_sq_q', 'scales'}: e4m3 codes of m and of sqrt(v) under one power of two
+                    per 128 elements (include/fsgs.h, fsgs_adamw_step); 2.02 bytes an element instead of 8.  `moments()`
+                    and `set_moments()` convert.  Changing a group's state_bits converts its moments at the next step.
+    master_weights  float32 copies of 16-bit parameters in state[p]['master'], which the step updates; the parameter is the
+                    copy rounded to nearest.  Made from the parameter at its first step.
+    maximize        ascend.
+    capturable      'step' is a 0-d float32 tensor on the parameter's device and lr may be one too, so that a step captured
+                    into a graph counts on at every replay.  A step of any other group inside a capture is refused.  Run one
+                    eager step before the capture: it makes the state.
+    max_grad_norm   bound on the 2-norm over the gradients of ALL groups (one device then): the step uses the gradients times
+                    min(1, max_grad_norm / (norm + 1e-6)) and leaves .grad as it is; `last_grad_norm` is that norm, 0-d on
+                    the device."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, maximize=False, state_bits=32,
+                 master_weights=False, capturable=False, max_grad_norm=None):
+        self.max_grad_norm = None if max_grad_norm is None else _max_norm(max_grad_norm)
+        self.last_grad_norm = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, maximize=maximize,
+                                      state_bits=state_bits, master_weights=master_weights, capturable=capturable))
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            self._scalars(group)
+            if len({id(p) for p in group["params"]}) != len(group["params"]):
+                raise ValueError("FusedAdamW: a parameter is given twice in one group")
+            for p in group["params"]:
+                if p.dtype not in _DTYPES:
+                    raise TypeError("FusedAdamW: float32, bfloat16 or float16 parameters, got %s" % p.dtype)
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self.__dict__.setdefault("max_grad_norm", None)
+        self.__dict__.setdefault("last_grad_norm", None)
+        for group in self.param_groups:  # groups saved by another Adam
+            for k, v in self.defaults.items():
+                group.setdefault(k, v)
+
+    @staticmethod
+    def _scalars(group):
+        """(lr, beta1, beta2, eps, weight_decay, lr tensor or None) of a group, checked"""
+        lr, lr_dev = group["lr"], None
+        if torch.is_tensor(lr):
+            if lr.numel() != 1:
+                raise ValueError("FusedAdamW: lr is a number or a tensor of one element")
+            if lr.is_cuda:
+                if not group["capturable"]:
+                    raise ValueError("FusedAdamW: lr as a tensor on the device needs capturable=True")
+                lr_dev, lr = lr, 0.0
+        lr, (b1, b2), eps, wd = float(lr), group["betas"], float(group["eps"]), float(group["weight_decay"])
+        b1, b2 = float(b1), float(b2)
+        for name, v, ok in (("lr", lr, lr >= 0), ("beta1", b1, 0 <= b1 < 1), ("beta2", b2, 0 <= b2 < 1), ("eps", eps, eps >= 0),
+                            ("weight_decay", wd, wd >= 0)):
+            if not ok:
+                raise ValueError("FusedAdamW: invalid %s: %r" % (name, v))
+        if group["state_bits"] not in (8, 32):
+            raise ValueError("FusedAdamW: state_bits is 8 or 32, got %r" % (group["state_bits"],))
+        return lr, b1, b2, eps, wd, lr_dev
+
+    # ---- state ------------------------------------------------------------------------------------------------------
+    @staticmethod
+    def _blocks(p):
+        return -(-p.numel() // _lib.ADAMW_BLOCK)
+
+    def _ready(self, p, st, group):
+        """the entries that the group's options ask for: made on the first step, converted where the options changed"""
+        if p.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("FusedAdamW: a parameter's state would be made inside a graph capture; run one eager step first")
+        like = dict(memory_format=torch.preserve_format)
+        if group["state_bits"] == 32 and "exp_avg" not in st:
+            if "exp_avg_q" in st:
+                self.widen(p)
+                st = self.state[p]
+            else:
+                st["exp_avg"], st["exp_avg_sq"] = torch.zeros_like(p, dtype=_F32, **like), torch.zeros_like(p, dtype=_F32, **like)
+        elif group["state_bits"] == 8 and "exp_avg_q" not in st:
+            if "exp_avg" in st:
+                self._write(p, st, st.pop("exp_avg"), st.pop("exp_avg_sq"))
+            else:
+                st["exp_avg_q"], st["exp_avg_sq_q"], st["scales"] = self._codes(p)
+        if group["master_weights"] and p.dtype != _F32 and "master" not in st:
+            st["master"] = p.detach().to(_F32, **like)
+        step = st.get("step", 0)
+        if group["capturable"]:
+            if not (torch.is_tensor(step) and step.device == p.device and step.dtype == _F32):
+                st["step"] = torch.full((), float(step), dtype=_F32, device=p.device)
+        else:
+            st["step"] = int(step)
+        return st
+
+    def _codes(self, p):
+        q = lambda: torch.empty_like(p, dtype=torch.uint8, memory_format=torch.preserve_format).zero_().view(_Q)  # noqa: E731
+        return q(), q(), torch.zeros((self._blocks(p), 2), dtype=torch.uint8, device=p.device)
+
+    def _state_tensors(self, p, st, bits):
+        """(m, v, scales or None), checked: raw pointers cross the C ABI"""
+        if bits == 32:
+            m, v, scales, want = st["exp_avg"], st["exp_avg_sq"], None, _F32
+        else:
+            m, v, scales, want = st["exp_avg_q"], st["exp_avg_sq_q"], st["scales"], _Q
+            if scales.dtype != torch.uint8 or scales.numel() != 2 * self._blocks(p) or not scales.is_contiguous() or \
+                    scales.device != p.device:
+                raise ValueError("FusedAdamW: state['scales'] is a contiguous uint8 [%d, 2] on %s" % (self._blocks(p), p.device))
+        if m.dtype != want or v.dtype != want or m.device != p.device or v.device != p.device or \
+                not _same_layout(m, p) or not _same_layout(v, p):
+            raise ValueError("FusedAdamW: the moments of a parameter are %s tensors of its shape and strides on its device; got "
+                             "%s %s and %s %s for %s" % (want, tuple(m.shape), m.dtype, tuple(v.shape), v.dtype, tuple(p.shape)))
+        return m, v, scales
+
+    def _read(self, items, dtype):
+        """values of 8-bit moments: one launch per 48 tensors of a device"""
+        lib, out, by_device = _lib.load(), [], {}
+        for p, st in items:
+            mq, vq, scales = self._state_tensors(p, st, 8)
+            if not p.is_cuda:
+                raise RuntimeError("FusedAdamW needs CUDA/HIP tensors; there is no CPU fallback")
+            m = torch.empty_like(mq, dtype=dtype, memory_format=torch.preserve_format)
+            v = torch.empty_like(mq, dtype=dtype, memory_format=torch.preserve_format)
+            out.append((m, v))
+            by_device.setdefault(p.device, array("q")).extend(
+                (mq.data_ptr(), vq.data_ptr(), scales.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel()))
+        for dev, table in by_device.items():
+            with _on(dev):
+                _lib.check(lib.fsgs_adamw_moments(len(table) // _lib.ADAMW_MOMENTS_WORDS, _address(table), 0, _DTYPES[dtype],
+                                                  _lib.current_stream()), "fsgs_adamw_moments")
+        return out
+
+    def _write(self, p, st, m, v):
+        lib = _lib.load()
+        if not p.is_cuda:
+            raise RuntimeError("FusedAdamW needs CUDA/HIP tensors; there is no CPU fallback")
+        if not _dense(p):
+            raise ValueError("FusedAdamW: parameters are dense in memory")
+        st["exp_avg_q"], st["exp_avg_sq_q"], st["scales"] = self._codes(p)
+        m, v = (torch.empty_like(p, dtype=_F32, memory_format=torch.preserve_format).copy_(x.detach()) for x in (m, v))
+        table = array("q", (st["exp_avg_q"].data_ptr(), st["exp_avg_sq_q"].data_ptr(), st["scales"].data_ptr(), m.data_ptr(),
+                            v.data_ptr(), p.numel()))
+        with _on(p.device):
+            _lib.check(lib.fsgs_adamw_moments(1, _address(table), 1, _lib.DTYPE_F32, _lib.current_stream()), "fsgs_adamw_moments")
+
+    @torch.no_grad()
+    def moments(self, dtype=torch.float32):
+        """[(m, v)] of every parameter that has a state, in the order of the groups: new tensors of the parameter's shape in
+        `dtype`.  float32 and bfloat16 hold what 8-bit moments stand for exactly."""
+        if dtype not in _DTYPES:
+            raise TypeError("moments: float32, bfloat16 or float16, got %s" % dtype)
+        items = [(p, self.state[p]) for group in self.param_groups for p in group["params"]
+                 if p in self.state and ("exp_avg" in self.state[p] or "exp_avg_q" in self.state[p])]
+        read = iter(self._read([it for it in items if "exp_avg_q" in it[1]], dtype))
+        return [next(read) if "exp_avg_q" in st else tuple(st[k].to(dtype, copy=True) for k in ("exp_avg", "exp_avg_sq"))
+                for _, st in items]
+
+    @torch.no_grad()
+    def widen(self, p):
+        """8-bit moments of parameter p as float32 'exp_avg' / 'exp_avg_sq' in its state (nothing to do where they are, or
+        where p has no state), for code that cuts or joins their rows; p's next step brings them back to the group's
+        state_bits"""
+        if "exp_avg_q" in self.state.get(p, {}):
+            self.state[p] = self.wide_state(p)
+
+    @torch.no_grad()
+    def wide_state(self, p):
+        """a copy of p's state entry (tensors shared) with float32 'exp_avg' / 'exp_avg_sq' whatever the moments' width, and
+        'step' as a number"""
+        st = dict(self.state[p])
+        if "step" in st and torch.is_tensor(st["step"]):
+            st["step"] = int(st["step"])
+        if "exp_avg_q" in st:
+            st["exp_avg"], st["exp_avg_sq"] = self._read([(p, st)], _F32)[0]
+            for k in ("exp_avg_q", "exp_avg_sq_q", "scales"):
+                del st[k]
+        return st
+
+    @torch.no_grad()
+    def set_moments(self, p, m, v, step):
+        """install values as the moments of parameter p (8-bit groups: rounded to the nearest codes) and its count of steps;
+        a 'master' that the state held is dropped and made again from p"""
+        group = next((g for g in self.param_groups if any(q is p for q in g["params"])), None)
+        if group is None:
+            raise ValueError("set_moments: not a parameter of this optimizer")
+        if m.shape != p.shape or v.shape != p.shape:
+            raise ValueError("set_moments: moments of shape %s and %s for a parameter of shape %s" % (
+                tuple(m.shape), tuple(v.shape), tuple(p.shape)))
+        st = {"step": step}
+        if group["state_bits"] == 8:
+            self._write(p, st, m, v)
+        else:
+            st["exp_avg"], st["exp_avg_sq"] = (
+                torch.empty_like(p, dtype=_F32, memory_format=torch.preserve_format).copy_(x.detach()) for x in (m, v))
+        self.state[p] = st
+        self._ready(p, st, group)
+
+    def load_state_dict(self, state_dict):
+        """as torch's, but every entry keeps its own type (torch casts floating state to the parameter's)"""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        mine = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, mine):
+            for k, v in state_dict["state"].get(i, {}).items():
+                if torch.is_tensor(v) and k != "step":
+                    self.state[p][k] = v.detach().to(p.device, copy=True)
+
+    # ---- the step -----------------------------------------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        lib = _lib.load()
+        capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
+        buckets, updated, keep = {}, [], []
+        for group in self.param_groups:
+            lr, b1, b2, eps, wd, lr_dev = self._scalars(group)
+            bits, masters, capturable = group["state_bits"], group["master_weights"], group["capturable"]
+            moment = "exp_avg" if bits == 32 else "exp_avg_q"
+            for p in group["params"]:
+                g = p.grad
+                if g is None:
+                    continue
+                dt, dev = p.dtype, p.device
+                if not p.is_cuda:
+                    raise RuntimeError("FusedAdamW needs CUDA/HIP tensors; there is no CPU fallback")
+                if g.layout != torch.strided:
+                    raise RuntimeError("FusedAdamW: sparse gradients are not supported")
+                if g.dtype != dt or g.device != dev:
+                    raise TypeError("FusedAdamW: a gradient has its parameter's type and device; got %s on %s for %s on %s" % (
+                        g.dtype, g.device, dt, dev))
+                if capturing and not capturable:
+                    raise RuntimeError("FusedAdamW: a step inside a graph capture needs capturable=True (its count and "
+                                       "learning rate would be frozen at every replay)")
+                if not (p.is_contiguous() and g.is_contiguous()):
+                    if not _dense(p):
+                        raise ValueError("FusedAdamW: parameters are dense in memory; got strides %s for %s" % (
+                            tuple(p.stride()), tuple(p.shape)))
+                    if not _same_layout(g, p):
+                        g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
+                        keep.append(g)
+                st = self.state[p]
+                use_master = masters and dt != _F32
+                step = st.get("step")
+                if moment not in st or step is None or (use_master and "master" not in st) or capturable != torch.is_tensor(step) or \
+                        (capturable and (step.device != dev or step.dtype != _F32)):
+                    st = self._ready(p, st, group)
+                m, v, scales = self._state_tensors(p, st, bits)
+                master = 0
+                if use_master:
+                    w = st["master"]
+                    if w.dtype != _F32 or w.device != dev or not _same_layout(w, p):
+                        raise ValueError("FusedAdamW: state['master'] is a float32 tensor of the parameter's shape and strides")
+                    master = w.data_ptr()
+                key = (dev, dt, bits, use_master, bool(group["maximize"]), bool(capturable))
+                table, hypers, index, counted = buckets.setdefault(key, (array("q"), [], {}, []))
+                if capturable:
+                    if lr_dev is not None and (lr_dev.device != dev or lr_dev.dtype != _F32):
+                        raise ValueError("FusedAdamW: lr as a tensor is float32 on the parameters' device")
+                    at = len(hypers)
+                    hypers.append((lr, b1, b2, eps, wd, 1, st["step"].data_ptr(), None if lr_dev is None else lr_dev.data_ptr()))
+                else:
+                    step = st["step"] + 1
+                    counted.append((st, step))
+                    hyper = (lr, b1, b2, eps, wd, step, None, None)
+                    at = index.get(hyper)
+                    if at is None:
+                        at = index[hyper] = len(hypers)
+                        hypers.append(hyper)
+                table.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(),
+                              0 if scales is None else scales.data_ptr(), master, p.numel(), at))
+                updated.append(p)
+        if not buckets:
+            return loss
+        coef = None
+        if self.max_grad_norm is not None:
+            grads = [p.grad for p in updated]
+            with _on(_one_device(grads, "FusedAdamW(max_grad_norm)")):
+                out = _norm_of(lib, grads, self.max_grad_norm)
+            self.last_grad_norm, coef = out[0], out[1:]
+        for (dev, dt, bits, _, maximize, capturable), (table, hypers, _, counted) in buckets.items():
+            n = len(table) // _lib.ADAMW_TENSOR_WORDS
+            with _on(dev):
+                scratch = None
+                if capturable:
+                    scratch = torch.empty(lib.fsgs_adamw_scratch_bytes(n), dtype=torch.uint8, device=dev)
+                rc = lib.fsgs_adamw_step(n, _address(table), len(hypers), (_lib.FsgsAdamWHyper * len(hypers))(*hypers),
+                                         _DTYPES[dt], bits, maximize, _lib.ptr(coef), _lib.ptr(scratch), _lib.current_stream())
+                if rc == _lib.FSGS_ERR_INVALID:
+                    raise ValueError("FusedAdamW: two of the tensors of a step share memory")
+                _lib.check(rc, "fsgs_adamw_step")
+            for st, step in counted:
+                st["step"] = step
+        mark_updated(updated)
+        return loss
 
 
 def densify_stats(radii, viewspace_grad, max_radii2D, xyz_gradient_accum, denom):

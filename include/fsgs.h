@@ -511,6 +511,70 @@ typedef struct FsgsAdamGroup {
 int fsgs_adam_step(int ngroups, const FsgsAdamGroup *groups, double beta1, double beta2, double eps,
                    fsgs_stream_t stream);
 
+/* AdamW (decoupled weight decay) over any number of tensors: up to 48 tensors and 8 different FsgsAdamWHyper a launch.
+ *   g' = grad_coef * grad (negated with maximize);  m = beta1 m + (1 - beta1) g';  v = beta2 v + (1 - beta2) g'^2
+ *   w = w (1 - lr weight_decay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * param and grad are of `dtype`; w is `master` (fp32) where given, and param = w rounded to nearest, else w is param itself.
+ * state_bits 32: exp_avg / exp_avg_sq are float[n].  state_bits 8: they are uint8[n] codes, OCP e4m3 of m / 2^E and of
+ * sqrt(v) / 2^E, and scales is uint8[ceil(n / 128)][2], E + 127 of both for each 128 consecutive elements (0 stands for a
+ * factor of 0, so all-zero state is valid).  New codes are rounded up or down by a threshold that belongs to the element
+ * and the step, evenly distributed over the steps; the step itself uses the moments before that rounding.
+ * Pointers need their element's alignment only.  No two tensors may share memory that is written. */
+#define FSGS_DTYPE_F32 0
+#define FSGS_DTYPE_BF16 1
+#define FSGS_DTYPE_F16 2
+#define FSGS_ADAMW_BLOCK 128
+typedef struct FsgsAdamWTensor {
+  void *param;
+  const void *grad;
+  void *exp_avg;
+  void *exp_avg_sq;
+  uint8_t *scales; /* state_bits 8 */
+  float *master;   /* or NULL; 16-bit dtype only; all tensors of a call or none */
+  int64_t n;
+  int64_t hyper;   /* index into hypers */
+} FsgsAdamWTensor;
+typedef struct FsgsAdamWHyper {
+  double lr, beta1, beta2, eps, weight_decay;
+  int64_t step;        /* 1-based count INCLUDING this step */
+  /* A step that a graph replays: step_dev float[1], the count BEFORE this step, incremented by the call, of one tensor alone
+   * (so one FsgsAdamWHyper a tensor); lr_dev float[1] or NULL (lr).  All tensors of a call or none. */
+  float *step_dev;
+  const float *lr_dev;
+} FsgsAdamWHyper;
+/* bytes of the scratch that a call with step_dev needs (kept until its kernels have run) */
+size_t fsgs_adamw_scratch_bytes(int n_tensors);
+/* tensors, hypers: HOST arrays.  grad_coef: float[1] DEVICE factor on the gradients (out2 + 1 of fsgs_grad_norm) or NULL.
+ * scratch: NULL without step_dev. */
+int fsgs_adamw_step(int n_tensors, const FsgsAdamWTensor *tensors, int n_hypers, const FsgsAdamWHyper *hypers, int dtype,
+                    int state_bits, int maximize, const float *grad_coef, void *scratch, fsgs_stream_t stream);
+/* 8-bit moments to values (write = 0; exp_avg / exp_avg_sq of `dtype`; bf16 and fp32 hold them exactly) or values (fp32) to
+ * codes, rounded to nearest (write = 1). */
+typedef struct FsgsAdamWMoments {
+  uint8_t *exp_avg_q;
+  uint8_t *exp_avg_sq_q;
+  uint8_t *scales;
+  void *exp_avg;
+  void *exp_avg_sq;
+  int64_t n;
+} FsgsAdamWMoments;
+int fsgs_adamw_moments(int n_tensors, const FsgsAdamWMoments *tensors, int write, int dtype, fsgs_stream_t stream);
+
+/* Global 2-norm of any number of gradients (squares summed in 64 bits, in a fixed order) and what bounds it:
+ * out2 float[2] DEVICE = {norm, min(1, max_norm / (norm + 1e-6))}; a NaN norm gives a NaN factor.  The same memory may
+ * be given twice (and counts twice).  scratch: fsgs_grad_norm_scratch_bytes(n_tensors), need not be cleared. */
+typedef struct FsgsGradTensor {
+  void *grad;
+  int64_t n;
+  int32_t dtype;
+  int32_t reserved;
+} FsgsGradTensor;
+size_t fsgs_grad_norm_scratch_bytes(int n_tensors);
+int fsgs_grad_norm(int n_tensors, const FsgsGradTensor *grads, float max_norm, void *scratch, size_t scratch_bytes,
+                   float *out2, fsgs_stream_t stream);
+/* grad *= coef[0] (DEVICE) in place, rounded to the gradient's type; a factor of exactly 1 moves no data. */
+int fsgs_grad_scale(int n_tensors, const FsgsGradTensor *grads, const float *coef, fsgs_stream_t stream);
+
 /* For every Gaussian with radii > 0: max_radii2D = max(., radii); xyz_gradient_accum += ||viewspace_grad||;
  * denom += 1   (scene/gaussian_model.py:678-681, train.py:298-303).  viewspace_grad [P,3]. */
 int fsgs_densify_stats(int P, const int32_t *radii, const float *viewspace_grad, float *max_radii2D,
