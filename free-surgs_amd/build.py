@@ -1,4 +1,5 @@
-"""Builds libfsgs_hip.so (all HIP kernels + the C ABI of include/fsgs.h) for gfx950, in-tree.
+"""Builds libfsgs_hip.so (all HIP kernels + the C ABI of include/fsgs.h) for gfx950, and _fsgs_host.so (the optimiser's walk
+over its tensors, a CPython extension for the torch at hand), in-tree.
 
     python free-surgs_amd/build.py [--force]
 
@@ -94,6 +95,32 @@ def _compile(src):
     return obj
 
 
+HOST_SRC = os.path.join(CSRC, "host.cpp")
+HOST_LIB = os.path.join(OUT_DIR, "_fsgs_host.so")
+
+
+def build_host():
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    inc = os.path.join(root, "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DNDEBUG",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I" + inc,
+           "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], HOST_SRC,
+           "-o", HOST_LIB, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    stamp, want = HOST_LIB.replace(".so", ".o.flags"), " ".join(cmd) + " " + torch.__version__
+    same = os.path.exists(stamp) and open(stamp).read() == want
+    if not same or _stale(HOST_LIB, [HOST_SRC, os.path.join(HERE, "..", "include", "fsgs.h")]):
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise RuntimeError("the host compiler failed for %s:\n%s\n%s" % (HOST_SRC, r.stdout, r.stderr))
+        with open(stamp, "w") as f:
+            f.write(want)
+    return HOST_LIB
+
+
 def build(force=False, verbose=False):
     os.makedirs(OBJ_DIR, exist_ok=True)
     if force:
@@ -101,7 +128,10 @@ def build(force=False, verbose=False):
             if f.endswith((".o", ".so", ".flags")):
                 os.remove(os.path.join(OBJ_DIR, f))
     with ThreadPoolExecutor(max_workers=4) as ex:
+        host = None if DIAG or TAG else ex.submit(build_host)
         objs = list(ex.map(_compile, sources()))
+        if host is not None:
+            host.result()
     if _stale(LIB, objs):
         cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
         r = subprocess.run(cmd, capture_output=True, text=True)

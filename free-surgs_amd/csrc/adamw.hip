@@ -617,7 +617,7 @@ int fsgs_adamw_step(int n_tensors, const FsgsAdamWTensor *tensors, int n_hypers,
       if (groups + chunks_of(x.n) > MAX_BLOCKS) break;
       int at = 0;
       if (!dev_h) {
-        while (at < n_used && used[at] != x.hyper) at++;
+        while (at < n_used && used[at] != x.hyper && std::memcmp(&hypers[used[at]], &hypers[x.hyper], sizeof(FsgsAdamWHyper))) at++;
         if (at == n_used) {
           if (n_used == HYPERS) break;
           const FsgsAdamWHyper &h = hypers[x.hyper];

@@ -243,6 +243,29 @@ def load():
     return _lib
 
 
+_host = None
+
+
+def host():
+    """The host extension (csrc/host.cpp); raises if it has not been built for this torch."""
+    global _host
+    if _host is None:
+        from importlib import machinery, util
+
+        path = os.path.join(_HERE, "lib", "_fsgs_host.so")
+        if not os.path.exists(path):
+            raise ImportError("_fsgs_host.so is missing (%s). Build it with `python free-surgs_amd/build.py`." % path)
+        import torch  # noqa: F401  (its libraries are what the extension links to)
+
+        with _lock:
+            if _host is None:
+                loader = machinery.ExtensionFileLoader("_fsgs_host", path)
+                mod = util.module_from_spec(util.spec_from_file_location("_fsgs_host", path, loader=loader))
+                loader.exec_module(mod)
+                _host = mod
+    return _host
+
+
 def check(code, where):
     if code != FSGS_OK:
         detail = ""

@@ -106,22 +106,36 @@ def _check_grad(g, name="gradient"):
         raise TypeError("%s: float32, bfloat16 or float16, got %s" % (name, g.dtype))
 
 
-def _norm_of(lib, grads, max_norm):
-    """(float32 [2] = {norm, factor}) of gradients on one device, on the current stream of that device"""
-    dev = grads[0].device
-    table, keep = array("q"), []
-    for g in grads:
-        if not _dense(g):
-            g = g.contiguous()
-            keep.append(g)
-        table.extend((g.data_ptr(), g.numel(), _DTYPES[g.dtype]))
-    n = len(grads)
+def _norm_of(lib, dev, table, max_norm):
+    """float32 [2] = {norm, factor} of the gradients in a table (rows of FsgsGradTensor), on dev's current stream"""
+    n = len(table) // _lib.GRAD_TENSOR_WORDS
     nbytes = lib.fsgs_grad_norm_scratch_bytes(n)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     out = torch.empty(2, dtype=_F32, device=dev)
-    _lib.check(lib.fsgs_grad_norm(n, _address(table), float(max_norm), scratch.data_ptr(), nbytes, out.data_ptr(),
+    _lib.check(lib.fsgs_grad_norm(n, _address(table), max_norm, scratch.data_ptr(), nbytes, out.data_ptr(),
                                   _lib.current_stream()), "fsgs_grad_norm")
     return out
+
+
+def _grad_table(params, grads, who):
+    """(device, rows, what to keep until the launch, gradients that are not dense) of the gradients of params"""
+    fast = _lib.host().grad_rows(params)
+    if fast is not None:
+        return torch.device("cuda", fast[1]), array("q", fast[0]), None, []
+    return _table_of(grads, who)
+
+
+def _table_of(grads, who):
+    dev, table, keep, strided = _one_device(grads, who), array("q"), [], []
+    for g in grads:
+        if g.is_neg():
+            raise RuntimeError("%s: a gradient is a negated view (resolve_neg)" % who)
+        if not _dense(g):
+            strided.append(g)
+            g = g.contiguous()
+            keep.append(g)
+        table.extend((g.data_ptr(), g.numel(), _DTYPES[g.dtype]))
+    return dev, table, keep, strided
 
 
 def _one_device(grads, who):
@@ -148,8 +162,9 @@ def grad_norm(tensors):
     if not tensors:
         return torch.tensor(0.0)
     lib = _lib.load()
-    with _on(_one_device(tensors, "grad_norm")):
-        return _norm_of(lib, tensors, float("inf"))[0]
+    dev, table, _keep, _ = _table_of(tensors, "grad_norm")
+    with _on(dev):
+        return _norm_of(lib, dev, table, float("inf"))[0]
 
 
 @torch.no_grad()
@@ -164,28 +179,28 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)
-    if len({id(g) for g in grads}) != len(grads):
-        raise ValueError("clip_grad_norm_: a parameter is given twice")
     lib = _lib.load()
-    dev = _one_device(grads, "clip_grad_norm_")
-    table, strided = array("q"), []
-    for g in grads:
-        if _dense(g):
-            table.extend((g.data_ptr(), g.numel(), _DTYPES[g.dtype]))
-        else:
-            strided.append(g)
+    dev, table, _keep, strided = _grad_table(parameters, grads, "clip_grad_norm_")
+    scaled = table
+    if strided:
+        if len({id(g) for g in grads}) != len(grads):
+            raise ValueError("clip_grad_norm_: a parameter is given twice")
+        scaled = _table_of([g for g in grads if _dense(g)], "clip_grad_norm_")[1] if len(strided) < len(grads) else array("q")
     with _on(dev):
-        out = _norm_of(lib, grads, max_norm)
+        out = _norm_of(lib, dev, table, max_norm)
         norm, coef = out[0], out[1]
         if error_if_nonfinite and not bool(torch.isfinite(norm)):
             raise RuntimeError("clip_grad_norm_: the gradients' norm is %s" % float(norm))
-        rc = lib.fsgs_grad_scale(len(table) // _lib.GRAD_TENSOR_WORDS, _address(table), coef.data_ptr(), _lib.current_stream())
+        rc = lib.fsgs_grad_scale(len(scaled) // _lib.GRAD_TENSOR_WORDS, _address(scaled), out.data_ptr() + 4, _lib.current_stream())
         if rc == _lib.FSGS_ERR_INVALID:
-            raise ValueError("clip_grad_norm_: two of the gradients share memory")
+            raise ValueError("clip_grad_norm_: two of the gradients share memory, or a parameter is given twice")
         _lib.check(rc, "fsgs_grad_scale")
         for g in strided:  # slices of other tensors; expanded ones torch itself refuses to write
             g.copy_(g.float() * coef)
-        mark_updated(grads)
+        if strided or _keep is not None:
+            mark_updated(grads)
+        else:
+            _lib.host().grads_written(parameters)
     return norm
 
 
@@ -312,6 +327,11 @@ class FusedAdamW(torch.optim.Optimizer):
     def _read(self, items, dtype):
         """values of 8-bit moments: one launch per 48 tensors of a device"""
         lib, out, by_device = _lib.load(), [], {}
+        fast = _lib.host().moment_rows([st for _, st in items], dtype) if items else None
+        if fast is not None and all(st["exp_avg_q"].shape == p.shape for p, st in items):
+            out, rows, index = fast
+            by_device[torch.device("cuda", index)] = array("q", rows)
+            items = ()
         for p, st in items:
             mq, vq, scales = self._state_tensors(p, st, 8)
             if not p.is_cuda:
@@ -410,11 +430,66 @@ class FusedAdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         lib = _lib.load()
+        work = self._ordinary()
+        if work is None:
+            work = self._general()
+        if not work:
+            return loss
+        coef = None
+        if self.max_grad_norm is not None:
+            params = [p for bucket in work for p in bucket.params]
+            dev, table, _keep, _ = _grad_table(params, [p.grad for p in params], "FusedAdamW(max_grad_norm)")
+            with _on(dev):
+                out = _norm_of(lib, dev, table, self.max_grad_norm)
+            self.last_grad_norm, coef = out[0], out.data_ptr() + 4
+        for b in work:
+            n = len(b.table) // _lib.ADAMW_TENSOR_WORDS
+            with _on(b.device):
+                scratch = torch.empty(lib.fsgs_adamw_scratch_bytes(n), dtype=torch.uint8, device=b.device) if b.capturable else None
+                rc = lib.fsgs_adamw_step(n, _address(b.table), len(b.hypers), (_lib.FsgsAdamWHyper * len(b.hypers))(*b.hypers),
+                                         b.dtype, b.bits, b.maximize, coef, _lib.ptr(scratch), _lib.current_stream())
+                if rc == _lib.FSGS_ERR_INVALID:
+                    raise ValueError("FusedAdamW: two of the tensors of a step share memory")
+                _lib.check(rc, "fsgs_adamw_step")
+            _lib.host().stepped(b.params, b.states)
+        return loss
+
+    def _ordinary(self):
+        """The buckets of a step whose tensors are all as one expects them -- packed, on one device, with their states in
+        place and counted alike within a group -- collected by the host extension; None where anything is not."""
+        by_key = {}
+        for group in self.param_groups:
+            if group["capturable"]:
+                return None
+            key = (group["state_bits"], bool(group["master_weights"]), bool(group["maximize"]))
+            lists, scalars = by_key.setdefault(key, ([], []))
+            lists.append(group["params"])
+            scalars.append(self._scalars(group)[:5])
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            return None
+        work, rows = [], _lib.host().step_rows
+        for (bits, masters, maximize), (lists, scalars) in by_key.items():
+            types = [-1]  # the first tensor's, then what else there is
+            for dtype in types:
+                found = rows(lists, self.state, bits, masters, dtype)
+                if found is None:
+                    return None
+                table, params, states, counts, code, others, index = found
+                if dtype < 0:
+                    types += [c for c in _DTYPES.values() if others >> c & 1]
+                if params:
+                    hypers = [(*h, c + 1 if c >= 0 else 1, None, None) for h, c in zip(scalars, counts)]
+                    work.append(_Bucket(torch.device("cuda", index), code, bits, maximize, False, array("q", table), hypers, params,
+                                        states))
+        return work
+
+    def _general(self):
+        """The buckets of any step that can be made: every tensor looked at in turn; states made or converted."""
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
-        buckets, updated, keep = {}, [], []
+        buckets = {}
         for group in self.param_groups:
             lr, b1, b2, eps, wd, lr_dev = self._scalars(group)
-            bits, masters, capturable = group["state_bits"], group["master_weights"], group["capturable"]
+            bits, masters, capturable = group["state_bits"], group["master_weights"], bool(group["capturable"])
             moment = "exp_avg" if bits == 32 else "exp_avg_q"
             for p in group["params"]:
                 g = p.grad
@@ -425,21 +500,23 @@ class FusedAdamW(torch.optim.Optimizer):
                     raise RuntimeError("FusedAdamW needs CUDA/HIP tensors; there is no CPU fallback")
                 if g.layout != torch.strided:
                     raise RuntimeError("FusedAdamW: sparse gradients are not supported")
-                if g.dtype != dt or g.device != dev:
+                if dt not in _DTYPES or g.dtype != dt or g.device != dev:
                     raise TypeError("FusedAdamW: a gradient has its parameter's type and device; got %s on %s for %s on %s" % (
                         g.dtype, g.device, dt, dev))
+                if p.is_neg() or g.is_neg():
+                    raise RuntimeError("FusedAdamW: a parameter or gradient is a negated view (resolve_neg)")
                 if capturing and not capturable:
                     raise RuntimeError("FusedAdamW: a step inside a graph capture needs capturable=True (its count and "
                                        "learning rate would be frozen at every replay)")
+                keep = None
                 if not (p.is_contiguous() and g.is_contiguous()):
                     if not _dense(p):
                         raise ValueError("FusedAdamW: parameters are dense in memory; got strides %s for %s" % (
                             tuple(p.stride()), tuple(p.shape)))
                     if not _same_layout(g, p):
-                        g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
-                        keep.append(g)
+                        g = keep = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
                 st = self.state[p]
-                use_master = masters and dt != _F32
+                use_master = bool(masters) and dt != _F32
                 step = st.get("step")
                 if moment not in st or step is None or (use_master and "master" not in st) or capturable != torch.is_tensor(step) or \
                         (capturable and (step.device != dev or step.dtype != _F32)):
@@ -451,47 +528,34 @@ class FusedAdamW(torch.optim.Optimizer):
                     if w.dtype != _F32 or w.device != dev or not _same_layout(w, p):
                         raise ValueError("FusedAdamW: state['master'] is a float32 tensor of the parameter's shape and strides")
                     master = w.data_ptr()
-                key = (dev, dt, bits, use_master, bool(group["maximize"]), bool(capturable))
-                table, hypers, index, counted = buckets.setdefault(key, (array("q"), [], {}, []))
+                key = (dev, dt, bits, use_master, bool(group["maximize"]), capturable)
+                b = buckets.get(key)
+                if b is None:
+                    b = buckets[key] = _Bucket(dev, _DTYPES[dt], bits, key[4], capturable, array("q"), [], [], [])
                 if capturable:
                     if lr_dev is not None and (lr_dev.device != dev or lr_dev.dtype != _F32):
                         raise ValueError("FusedAdamW: lr as a tensor is float32 on the parameters' device")
-                    at = len(hypers)
-                    hypers.append((lr, b1, b2, eps, wd, 1, st["step"].data_ptr(), None if lr_dev is None else lr_dev.data_ptr()))
+                    hyper = (lr, b1, b2, eps, wd, 1, st["step"].data_ptr(), None if lr_dev is None else lr_dev.data_ptr())
                 else:
-                    step = st["step"] + 1
-                    counted.append((st, step))
-                    hyper = (lr, b1, b2, eps, wd, step, None, None)
-                    at = index.get(hyper)
-                    if at is None:
-                        at = index[hyper] = len(hypers)
-                        hypers.append(hyper)
-                table.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(),
-                              0 if scales is None else scales.data_ptr(), master, p.numel(), at))
-                updated.append(p)
-        if not buckets:
-            return loss
-        coef = None
-        if self.max_grad_norm is not None:
-            grads = [p.grad for p in updated]
-            with _on(_one_device(grads, "FusedAdamW(max_grad_norm)")):
-                out = _norm_of(lib, grads, self.max_grad_norm)
-            self.last_grad_norm, coef = out[0], out[1:]
-        for (dev, dt, bits, _, maximize, capturable), (table, hypers, _, counted) in buckets.items():
-            n = len(table) // _lib.ADAMW_TENSOR_WORDS
-            with _on(dev):
-                scratch = None
-                if capturable:
-                    scratch = torch.empty(lib.fsgs_adamw_scratch_bytes(n), dtype=torch.uint8, device=dev)
-                rc = lib.fsgs_adamw_step(n, _address(table), len(hypers), (_lib.FsgsAdamWHyper * len(hypers))(*hypers),
-                                         _DTYPES[dt], bits, maximize, _lib.ptr(coef), _lib.ptr(scratch), _lib.current_stream())
-                if rc == _lib.FSGS_ERR_INVALID:
-                    raise ValueError("FusedAdamW: two of the tensors of a step share memory")
-                _lib.check(rc, "fsgs_adamw_step")
-            for st, step in counted:
-                st["step"] = step
-        mark_updated(updated)
-        return loss
+                    hyper = (lr, b1, b2, eps, wd, st["step"] + 1, None, None)
+                at = b.index.setdefault(hyper, len(b.hypers))
+                if at == len(b.hypers):
+                    b.hypers.append(hyper)
+                b.table.extend((p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(),
+                                0 if scales is None else scales.data_ptr(), master, p.numel(), at))
+                b.keep.append(keep)
+                b.params.append(p)
+                b.states.append(st)
+        return list(buckets.values())
+
+
+class _Bucket:
+    """tensors of one launch sequence: one device, type, width of the moments and direction"""
+
+    def __init__(self, device, dtype, bits, maximize, capturable, table, hypers, params, states):
+        self.device, self.dtype, self.bits, self.maximize, self.capturable = device, dtype, bits, maximize, capturable
+        self.table, self.hypers, self.params, self.states = table, hypers, params, states
+        self.index, self.keep = {}, []
 
 
 def densify_stats(radii, viewspace_grad, max_radii2D, xyz_gradient_accum, denom):

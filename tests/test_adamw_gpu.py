@@ -501,6 +501,40 @@ def test_the_norm_bound_inside_a_step_is_the_clip_in_front_of_it():
             close(opt.state[p]["exp_avg"], m1, tm, "m"), close(opt.state[p]["exp_avg_sq"], v1, tv, "v")
 
 
+@pytest.mark.parametrize("bits,masters", [(32, False), (8, True)])
+def test_the_quick_walk_gives_what_the_general_one_gives(bits, masters, monkeypatch):
+    """a step collected by the host extension against one collected tensor by tensor: groups of other options and types,
+    parameters without gradients, more groups than a launch has scalars"""
+    def build():
+        ps = sum((make([5, 700, 4099, 1], dtype, seed=70)[0] for dtype in DTYPES), [])
+        groups = [{"params": [p], "lr": 1e-3 * (1 + i % 9), "betas": (0.9, 0.99 if i % 4 else 0.9)} for i, p in enumerate(ps)]
+        groups[3]["state_bits"], groups[5]["maximize"], groups[7]["weight_decay"] = 40 - bits, True, 0.3
+        return ps, FusedAdamW(groups, state_bits=bits, master_weights=masters, max_grad_norm=0.2)
+
+    (ps, a), (qs, b) = build(), build()
+    quick = []
+    ordinary = FusedAdamW._ordinary
+    for k in range(4):
+        for i, (p, q) in enumerate(zip(ps, qs)):
+            g = torch.randn(p.shape, generator=torch.Generator().manual_seed(100 * k + i)).to(DEV, p.dtype)
+            p.grad, q.grad = (None, None) if (i + k) % 5 == 0 and k < 3 else (g, g.clone())
+        monkeypatch.setattr(FusedAdamW, "_ordinary", lambda self: quick.append(ordinary(self)) or quick[-1])
+        versions = [p._version for p in ps]
+        a.step()
+        assert all((p._version > v) == (p.grad is not None) for p, v in zip(ps, versions))
+        monkeypatch.setattr(FusedAdamW, "_ordinary", lambda self: None)
+        b.step()
+    assert quick[0] is None and quick[-1] is not None
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q) and a.state[p]["step"] == b.state[q]["step"]
+        for k, v in a.state[p].items():
+            if torch.is_tensor(v):
+                assert torch.equal(v.view(torch.uint8) if v.dtype == torch.float8_e4m3fn else v,
+                                   b.state[q][k].view(torch.uint8) if v.dtype == torch.float8_e4m3fn else b.state[q][k]), k
+    for (m, v), (m2, v2) in zip(a.moments(), b.moments()):
+        assert torch.equal(m, m2) and torch.equal(v, v2)
+
+
 def test_streams_and_steps_behind_each_other():
     ps, gs = make([200000], torch.float32, seed=40)
     qs = [p.detach().clone().requires_grad_(True) for p in ps]
