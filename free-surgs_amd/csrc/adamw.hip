@@ -5,7 +5,11 @@
 //   w  = w (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // A few dozen operations an element against 16 to 30 bytes: everything here is bound by HBM, so each kernel reads and writes
-// every array once, with 16-byte accesses where the type allows, and one launch takes up to 48 tensors.
+// every array once, with 16-byte accesses where the type allows, and one launch takes up to 48 tensors (192 gradients).
+// The step's loads and stores are non-temporal, what they move is next used a whole step later: 1 M Gaussians (59 M floats)
+// 311 -> 280 us (5.9 TB/s) with 32-bit moments, 176 -> 155 us (6.1 TB/s) with 8-bit ones; on the loads or on the stores
+// alone there is next to nothing to gain (302 and 313 us).  The norm's and the scaling's are not: gradients come from a
+// cache as often as not (20 M bf16: 15.6 us against 17.7).
 //
 // Which tensor a workgroup belongs to: lane k of every wave compares the workgroup's number with the first workgroup of
 // tensor k, and the number of lanes at or past theirs is the answer -- one load and one ballot, no search.
@@ -36,9 +40,15 @@ using namespace fsgs;
 namespace {
 
 constexpr int TENSORS = 48;            // of one launch: the table is a kernel argument, 4 KB at most
+constexpr int GRADS = 192;             // of one norm or scaling launch
 constexpr int HYPERS = 8;              // different sets of scalars of one launch
 constexpr int THREADS = 256;
-constexpr int CHUNK = 4096;            // elements of one workgroup
+// Elements of one workgroup of a step: two vectors a thread and array.  Four make fewer, larger workgroups (20 k Gaussians,
+// 1.2 M floats: 10.1 us against 8.1; 24 bf16 layers of 20 M in 8 bits: 59 us against 54; no difference at 59 M).
+constexpr int CHUNK = 2048;
+// Bytes of one workgroup's turn: four 16-byte vectors a thread in the norm, two in the scaling (160 bf16 layers of 64 M: norm
+// 27.6 us, with two 30.9, with eight 28.5; scaling 48.0 us, with four 51.7, with one 60.1).
+constexpr int NORM_BYTES = 16384, SCALE_BYTES = 8192;
 constexpr int64_t MAX_BLOCKS = 1 << 23;  // workgroups of one launch (256 threads each: 2^31 work items)
 constexpr int QBLOCK = FSGS_ADAMW_BLOCK;  // elements that share a power of two
 constexpr int NORM_GROUPS = 2048;      // workgroups of one norm launch at most: eight per CU
@@ -72,27 +82,42 @@ __host__ __device__ inline Hyper make_hyper(double lr, double b1, double b2, dou
   return h;
 }
 
+// a tensor's entry is one aligned 64 bytes: arguments are read from the host's memory the first time, line by line
+struct Entry {
+  void *p;
+  const void *g;
+  void *m, *v;
+  void *w;          // fp32 master weights
+  uint8_t *scales;
+  int64_t n;
+  uint32_t start;   // first workgroup (as in Table::start)
+  uint32_t hyper;
+};
 struct Table {
-  void *p[TENSORS];
-  const void *g[TENSORS];
-  void *m[TENSORS], *v[TENSORS];
-  void *w[TENSORS];        // fp32 master weights
-  uint8_t *scales[TENSORS];
-  int64_t n[TENSORS];
-  uint32_t start[TENSORS];  // first workgroup
-  uint8_t hyper[TENSORS];
-  Hyper h[HYPERS];
-  const Hyper *dev_h;       // one per tensor, or NULL: h[hyper[k]]
-  const float *coef;        // factor on the gradients, or NULL
+  uint32_t start[TENSORS];
   int count;
   float sign;               // -1: ascend
+  const Hyper *dev_h;       // one per tensor, or NULL: h[hyper]
+  const float *coef;        // factor on the gradients, or NULL
+  Hyper h[HYPERS];
+  alignas(64) Entry at[TENSORS];
 };
-static_assert(sizeof(Table) <= 4096, "kernel argument");
+static_assert(sizeof(Table) <= 4096 && sizeof(Entry) == 64, "kernel argument");
 
-__device__ __forceinline__ int owner(const uint32_t *start, int count, uint32_t group) {
+template <int MAX> __device__ __forceinline__ int owner(const uint32_t *start, int count, uint32_t group) {
   const int lane = threadIdx.x & 63;
-  const bool at = lane < count && group >= start[lane < TENSORS ? lane : TENSORS - 1];
-  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(at)) - 1);
+  int k = -1;
+#pragma unroll
+  for (int first = 0; first < MAX; first += 64) {
+    if (first > 0 && count <= first) break;
+    const int at = first + lane;
+    k += __popcll(__ballot(at < count && group >= start[at < MAX ? at : MAX - 1]));
+  }
+  return __builtin_amdgcn_readfirstlane(k);
+}
+__device__ __forceinline__ Hyper hyper_of(const Table &t, int k) {
+  if (t.dev_h) return t.dev_h[k];
+  return t.h[t.at[k].hyper];
 }
 
 // vectors of four that need only their element's alignment: the hardware's wide global accesses ask for no more
@@ -106,24 +131,30 @@ template <> struct Vec4<float> { typedef float4u type; };
 template <> struct Vec4<__bf16> { typedef bf4u type; };
 template <> struct Vec4<_Float16> { typedef half4u type; };
 
-template <typename T> __device__ __forceinline__ void load4(const T *at, float (&x)[4]) {
-  const typename Vec4<T>::type a = *(const typename Vec4<T>::type *)at;
+template <bool STREAM, typename T> __device__ __forceinline__ void load4(const T *at, float (&x)[4]) {
+  typename Vec4<T>::type a;
+  if constexpr (STREAM) a = __builtin_nontemporal_load((const typename Vec4<T>::type *)at);
+  else a = *(const typename Vec4<T>::type *)at;
 #pragma unroll
   for (int j = 0; j < 4; j++) x[j] = (float)a[j];
 }
-template <typename T> __device__ __forceinline__ void store4(T *at, const float (&x)[4]) {
+template <bool STREAM, typename T> __device__ __forceinline__ void store4(T *at, const float (&x)[4]) {
   typename Vec4<T>::type a;
 #pragma unroll
   for (int j = 0; j < 4; j++) a[j] = (T)x[j];  // one rounding to the parameter's type, to nearest even
-  *(typename Vec4<T>::type *)at = a;
+  if constexpr (STREAM) __builtin_nontemporal_store(a, (typename Vec4<T>::type *)at);
+  else *(typename Vec4<T>::type *)at = a;
 }
+// the first `have` of four elements: a tensor's last workgroup
 template <typename T> __device__ __forceinline__ void load_some(const T *at, float (&x)[4], int have) {
+  if (have >= 4) return load4<false>(at, x);
 #pragma unroll
   for (int j = 0; j < 4; j++) x[j] = j < have ? (float)at[j] : 0.0f;
 }
 template <typename T> __device__ __forceinline__ void store_some(T *at, const float (&x)[4], int have) {
+  if (have >= 4) return store4<false>(at, x);
 #pragma unroll
-  for (int j = 0; j < 4; j++)
+  for (int j = 0; j < 3; j++)
     if (j < have) at[j] = (T)x[j];
 }
 
@@ -135,22 +166,23 @@ __device__ __forceinline__ void adamw_one(float &w, float g, float &m, float &v,
 }
 
 template <typename T, bool MASTER> __global__ __launch_bounds__(THREADS) void adamw32_kernel(Table t) {
-  const int k = owner(t.start, t.count, blockIdx.x);
-  const Hyper h = t.dev_h ? t.dev_h[k] : t.h[t.hyper[k]];
+  const int k = owner<TENSORS>(t.start, t.count, blockIdx.x);
+  const Entry &e = t.at[k];
+  const Hyper h = hyper_of(t, k);
   const float scale = t.sign * (t.coef ? *t.coef : 1.0f);
-  const int64_t base = (int64_t)(blockIdx.x - t.start[k]) * CHUNK;
-  const int64_t left = t.n[k] - base;
-  T *p = (T *)t.p[k] + base;
-  const T *g = (const T *)t.g[k] + base;
-  float *m = (float *)t.m[k] + base, *v = (float *)t.v[k] + base, *w = MASTER ? (float *)t.w[k] + base : nullptr;
+  const int64_t base = (int64_t)(blockIdx.x - e.start) * CHUNK;
+  const int64_t left = e.n - base;
+  T *p = (T *)e.p + base;
+  const T *g = (const T *)e.g + base;
+  float *m = (float *)e.m + base, *v = (float *)e.v + base, *w = MASTER ? (float *)e.w + base : nullptr;
   constexpr int U = CHUNK / (THREADS * 4);
   float ww[U][4], gg[U][4], mm[U][4], vv[U][4];
   if (left >= CHUNK) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int i = (u * THREADS + threadIdx.x) * 4;
-      load4(g + i, gg[u]); load4(m + i, mm[u]); load4(v + i, vv[u]);
-      if constexpr (MASTER) load4(w + i, ww[u]); else load4(p + i, ww[u]);
+      load4<false>(g + i, gg[u]); load4<true>(m + i, mm[u]); load4<true>(v + i, vv[u]);
+      if constexpr (MASTER) load4<true>(w + i, ww[u]); else load4<true>(p + i, ww[u]);
     }
   } else {
 #pragma unroll
@@ -168,8 +200,8 @@ template <typename T, bool MASTER> __global__ __launch_bounds__(THREADS) void ad
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int i = (u * THREADS + threadIdx.x) * 4;
-      store4(p + i, ww[u]); store4(m + i, mm[u]); store4(v + i, vv[u]);
-      if constexpr (MASTER) store4(w + i, ww[u]);
+      store4<true>(p + i, ww[u]); store4<true>(m + i, mm[u]); store4<true>(v + i, vv[u]);
+      if constexpr (MASTER) store4<true>(w + i, ww[u]);
     }
   } else {
 #pragma unroll
@@ -251,15 +283,16 @@ __device__ __forceinline__ void adamw8_one(float &w, float g, float &m, float &r
 }
 
 template <typename T, bool MASTER> __global__ __launch_bounds__(THREADS) void adamw8_kernel(Table t) {
-  const int k = owner(t.start, t.count, blockIdx.x);
-  const Hyper h = t.dev_h ? t.dev_h[k] : t.h[t.hyper[k]];
+  const int k = owner<TENSORS>(t.start, t.count, blockIdx.x);
+  const Entry &e = t.at[k];
+  const Hyper h = hyper_of(t, k);
   const float scale = t.sign * (t.coef ? *t.coef : 1.0f);
-  const int64_t base = (int64_t)(blockIdx.x - t.start[k]) * CHUNK;
-  const int left = (int)min(t.n[k] - base, (int64_t)CHUNK);
-  T *p = (T *)t.p[k] + base;
-  const T *g = (const T *)t.g[k] + base;
-  uint8_t *m = (uint8_t *)t.m[k] + base, *r = (uint8_t *)t.v[k] + base, *scales = t.scales[k] + 2 * (base / QBLOCK);
-  float *w = MASTER ? (float *)t.w[k] + base : nullptr;
+  const int64_t base = (int64_t)(blockIdx.x - e.start) * CHUNK;
+  const int left = (int)min(e.n - base, (int64_t)CHUNK);
+  T *p = (T *)e.p + base;
+  const T *g = (const T *)e.g + base;
+  uint8_t *m = (uint8_t *)e.m + base, *r = (uint8_t *)e.v + base, *scales = e.scales + 2 * (base / QBLOCK);
+  float *w = MASTER ? (float *)e.w + base : nullptr;
   constexpr int U = CHUNK / (THREADS * 8);
   // block of this lane and its first element in it
   const int row = threadIdx.x / 16, at = (threadIdx.x & 15) * 4;
@@ -273,8 +306,8 @@ template <typename T, bool MASTER> __global__ __launch_bounds__(THREADS) void ad
     for (int s = 0; s < 2; s++) {
       const int i = b * QBLOCK + s * 64 + at;
       if (left == CHUNK) {
-        load4(g + i, gg[u][s]);
-        if constexpr (MASTER) load4(w + i, ww[u][s]); else load4(p + i, ww[u][s]);
+        load4<false>(g + i, gg[u][s]);
+        if constexpr (MASTER) load4<true>(w + i, ww[u][s]); else load4<true>(p + i, ww[u][s]);
         mq[u][s] = *(const u32u *)(m + i);
         rq[u][s] = *(const u32u *)(r + i);
       } else {
@@ -307,12 +340,12 @@ template <typename T, bool MASTER> __global__ __launch_bounds__(THREADS) void ad
 #pragma unroll
     for (int s = 0; s < 2; s++) {
       const int i = b * QBLOCK + s * 64 + at;
-      const uint32_t e = (uint32_t)base + (uint32_t)i;
-      const uint32_t cm = codes_of<false>(mm[s], inv_m, e * PHASE_M + h.shift_m, PHASE_M);
-      const uint32_t cr = codes_of<true>(rr[s], inv_r, e * PHASE_R + h.shift_r, PHASE_R);
+      const uint32_t place = (uint32_t)base + (uint32_t)i;
+      const uint32_t cm = codes_of<false>(mm[s], inv_m, place * PHASE_M + h.shift_m, PHASE_M);
+      const uint32_t cr = codes_of<true>(rr[s], inv_r, place * PHASE_R + h.shift_r, PHASE_R);
       if (left == CHUNK) {
-        store4(p + i, ww[u][s]);
-        if constexpr (MASTER) store4(w + i, ww[u][s]);
+        store4<true>(p + i, ww[u][s]);
+        if constexpr (MASTER) store4<true>(w + i, ww[u][s]);
         *(u32u *)(m + i) = cm;
         *(u32u *)(r + i) = cr;
       } else {
@@ -337,7 +370,7 @@ static_assert(sizeof(MomentTable) <= 4096, "kernel argument");
 
 // v = r^2 of a four-bit code has eight significant bits: bf16 holds m and v exactly (within its range)
 template <typename T> __global__ __launch_bounds__(THREADS) void moments_read_kernel(MomentTable t) {
-  const int k = owner(t.start, t.count, blockIdx.x);
+  const int k = owner<TENSORS>(t.start, t.count, blockIdx.x);
   const int64_t base = (int64_t)(blockIdx.x - t.start[k]) * CHUNK;
   const int left = (int)min(t.n[k] - base, (int64_t)CHUNK);
   const uint8_t *mq = t.mq[k] + base, *rq = t.rq[k] + base, *scales = t.scales[k] + 2 * (base / QBLOCK);
@@ -354,7 +387,7 @@ template <typename T> __global__ __launch_bounds__(THREADS) void moments_read_ke
 #pragma unroll
     for (int j = 0; j < 4; j++) rr[j] = rr[j] * rr[j];
     if (have >= 4) {
-      store4(m + i, mm); store4(v + i, rr);
+      store4<true>(m + i, mm); store4<true>(v + i, rr);
     } else {
       store_some(m + i, mm, have); store_some(v + i, rr, have);
     }
@@ -363,7 +396,7 @@ template <typename T> __global__ __launch_bounds__(THREADS) void moments_read_ke
 
 // values to codes, to nearest (the threshold is one half for every element)
 __global__ __launch_bounds__(THREADS) void moments_write_kernel(MomentTable t) {
-  const int k = owner(t.start, t.count, blockIdx.x);
+  const int k = owner<TENSORS>(t.start, t.count, blockIdx.x);
   const int64_t base = (int64_t)(blockIdx.x - t.start[k]) * CHUNK;
   const int left = (int)min(t.n[k] - base, (int64_t)CHUNK);
   uint8_t *mq = t.mq[k] + base, *rq = t.rq[k] + base, *scales = t.scales[k] + 2 * (base / QBLOCK);
@@ -417,87 +450,114 @@ __global__ __launch_bounds__(64) void adamw_scalars_kernel(ScalarTable t) {
 
 // ---- global norm --------------------------------------------------------------------------------------------------------
 struct GradTable {
-  void *g[TENSORS];
-  int64_t n[TENSORS];
-  uint32_t start[TENSORS + 1];  // first chunk
-  uint8_t dtype[TENSORS];
+  uint32_t start[GRADS];  // first turn
+  uint32_t turns;
   int count;
+  struct { void *g; int64_t n_dtype; } at[GRADS];  // n << 2 | dtype
 };
 static_assert(sizeof(GradTable) <= 4096, "kernel argument");
 
-template <typename T> __device__ __forceinline__ double chunk_squares(const T *g, int64_t left) {
-  constexpr int U = CHUNK / (THREADS * 4);
-  float x[U][4];
+// two bytes an element: eight of them make 16 bytes
+typedef __bf16 bf8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef _Float16 half8u __attribute__((ext_vector_type(8), aligned(2)));
+typedef float float4r __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8r __attribute__((ext_vector_type(8)));
+typedef _Float16 half8r __attribute__((ext_vector_type(8)));
+template <typename T> struct Vec16;  // in memory, in registers
+template <> struct Vec16<float> { typedef float4u mem; typedef float4r reg; };
+template <> struct Vec16<__bf16> { typedef bf8u mem; typedef bf8r reg; };
+template <> struct Vec16<_Float16> { typedef half8u mem; typedef half8r reg; };
+
+// one turn of a workgroup: F(vector) of up to BYTES of a tensor that has `left` bytes from `g` on, stored again with WRITE
+template <typename T, int BYTES, bool WRITE, typename F> __device__ __forceinline__ void turn(T *g, int64_t left, F f) {
+  typedef typename Vec16<T>::mem M;
+  typedef typename Vec16<T>::reg V;
+  constexpr int L = 16 / sizeof(T), U = BYTES / (THREADS * 16);
+  V x[U];
+  if (left >= BYTES) {
+#pragma unroll
+    for (int u = 0; u < U; u++) x[u] = *(const M *)(g + (u * THREADS + threadIdx.x) * L);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      f(x[u]);
+      if constexpr (WRITE) *(M *)(g + (u * THREADS + threadIdx.x) * L) = x[u];
+    }
+    return;
+  }
+  const int n = (int)(left / (int)sizeof(T));
 #pragma unroll
   for (int u = 0; u < U; u++) {
-    const int i = (u * THREADS + threadIdx.x) * 4;
-    if (left >= CHUNK) load4(g + i, x[u]);
-    else load_some(g + i, x[u], (int)left - i);
-  }
-  double a = 0.0, b = 0.0;
+    const int i = (u * THREADS + threadIdx.x) * L;
+    x[u] = V{};
+    if (i + L <= n) x[u] = *(const M *)(g + i);
+    else
 #pragma unroll
-  for (int u = 0; u < U; u++) {
-    a = fma((double)x[u][0], (double)x[u][0], a); b = fma((double)x[u][1], (double)x[u][1], b);
-    a = fma((double)x[u][2], (double)x[u][2], a); b = fma((double)x[u][3], (double)x[u][3], b);
+      for (int j = 0; j < L; j++)
+        if (i + j < n) x[u][j] = g[i + j];
+    f(x[u]);
+    if constexpr (WRITE) {
+      if (i + L <= n) *(M *)(g + i) = x[u];
+      else
+#pragma unroll
+        for (int j = 0; j < L; j++)
+          if (i + j < n) g[i + j] = x[u][j];
+    }
   }
-  return a + b;
+}
+template <int BYTES, bool WRITE, typename F>
+__device__ __forceinline__ void turn_of(const GradTable &t, int k, uint32_t at, F f) {
+  const int64_t nd = t.at[k].n_dtype, n = nd >> 2, done = (int64_t)(at - t.start[k]) * BYTES;
+  char *g = (char *)t.at[k].g + done;
+  if ((nd & 3) == FSGS_DTYPE_F32) turn<float, BYTES, WRITE>((float *)g, 4 * n - done, f);
+  else if ((nd & 3) == FSGS_DTYPE_BF16) turn<__bf16, BYTES, WRITE>((__bf16 *)g, 2 * n - done, f);
+  else turn<_Float16, BYTES, WRITE>((_Float16 *)g, 2 * n - done, f);
 }
 
-__device__ __forceinline__ double group_sum(double a, double *lds) {  // valid in thread 0
+template <int WAVES> __device__ __forceinline__ double group_sum(double a, double *lds) {  // the same in every thread of wave 0
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) a += __shfl_down(a, d, 64);
-  const int wave = threadIdx.x >> 6;
-  if ((threadIdx.x & 63) == 0) lds[wave] = a;
+  for (int d = 32; d > 0; d >>= 1) a += __shfl_xor(a, d, 64);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
   __syncthreads();
   double s = lds[0];
-  for (int k = 1; k < THREADS / 64; k++) s += lds[k];
+#pragma unroll
+  for (int k = 1; k < WAVES; k++) s += lds[k];
   return s;
 }
 
-// Squares are summed in 64 bits (no overflow, no loss over long sums), each workgroup over its own chunks in a fixed order:
-// the same gradients give the same norm to the last bit.
-__global__ __launch_bounds__(THREADS) void norm_partial_kernel(GradTable t, double *partial) {
-  __shared__ double lds[THREADS / 64];
-  double sum = 0.0;
-  for (uint32_t c = blockIdx.x; c < t.start[t.count]; c += gridDim.x) {
-    const int k = owner(t.start, t.count, c);
-    const int64_t base = (int64_t)(c - t.start[k]) * CHUNK, left = t.n[k] - base;
-    if (t.dtype[k] == FSGS_DTYPE_F32) sum += chunk_squares((const float *)t.g[k] + base, left);
-    else if (t.dtype[k] == FSGS_DTYPE_BF16) sum += chunk_squares((const __bf16 *)t.g[k] + base, left);
-    else sum += chunk_squares((const _Float16 *)t.g[k] + base, left);
+struct Squares {
+  double a = 0.0, b = 0.0;
+  template <typename V> __device__ __forceinline__ void operator()(const V &x) {
+    constexpr int L = sizeof(V) / sizeof(x[0]);
+#pragma unroll
+    for (int j = 0; j < L; j += 2) {
+      const double p = (double)(float)x[j], q = (double)(float)x[j + 1];
+      a = fma(p, p, a);
+      b = fma(q, q, b);
+    }
   }
-  const double s = group_sum(sum, lds);
+};
+
+// Squares are summed in 64 bits (no overflow, no loss over long sums), each workgroup over its own turns in a fixed order:
+// the same gradients give the same norm to the last bit.
+__global__ __launch_bounds__(THREADS, 8) void norm_partial_kernel(GradTable t, double *partial) {
+  __shared__ double lds[THREADS / 64];
+  Squares sum;
+  for (uint32_t at = blockIdx.x; at < t.turns; at += gridDim.x)
+    turn_of<NORM_BYTES, false>(t, owner<GRADS>(t.start, t.count, at), at, [&](const auto &x) { sum(x); });
+  const double s = group_sum<THREADS / 64>(sum.a + sum.b, lds);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
-__global__ __launch_bounds__(THREADS) void norm_finish_kernel(const double *partial, int count, float max_norm, float *out2) {
-  __shared__ double lds[THREADS / 64];
+__global__ __launch_bounds__(1024) void norm_finish_kernel(const double *partial, int count, float max_norm, float *norm_out,
+                                                              float *factor) {
+  __shared__ double lds[16];
   double sum = 0.0;
-  for (int i = threadIdx.x; i < count; i += THREADS) sum += partial[i];
-  const double s = group_sum(sum, lds);
+  for (int i = threadIdx.x; i < count; i += 1024) sum += partial[i];
+  const double s = group_sum<16>(sum, lds);
   if (threadIdx.x == 0) {
     const float norm = (float)sqrt(s), c = max_norm / (norm + 1e-6f);
-    out2[0] = norm;
-    out2[1] = c > 1.0f ? 1.0f : c;  // NaN stays NaN
-  }
-}
-
-template <typename T> __device__ __forceinline__ void chunk_scale(T *g, int64_t left, float c) {
-  constexpr int U = CHUNK / (THREADS * 4);
-  float x[U][4];
-#pragma unroll
-  for (int u = 0; u < U; u++) {
-    const int i = (u * THREADS + threadIdx.x) * 4;
-    if (left >= CHUNK) load4(g + i, x[u]);
-    else load_some(g + i, x[u], (int)left - i);
-  }
-#pragma unroll
-  for (int u = 0; u < U; u++) {
-    const int i = (u * THREADS + threadIdx.x) * 4;
-#pragma unroll
-    for (int j = 0; j < 4; j++) x[u][j] *= c;
-    if (left >= CHUNK) store4(g + i, x[u]);
-    else store_some(g + i, x[u], (int)left - i);
+    *norm_out = norm;
+    *factor = c > 1.0f ? 1.0f : c;  // NaN stays NaN
   }
 }
 
@@ -505,11 +565,10 @@ template <typename T> __device__ __forceinline__ void chunk_scale(T *g, int64_t 
 __global__ __launch_bounds__(THREADS) void grad_scale_kernel(GradTable t, const float *coef) {
   const float c = *coef;
   if (c == 1.0f) return;
-  const int k = owner(t.start, t.count, blockIdx.x);
-  const int64_t base = (int64_t)(blockIdx.x - t.start[k]) * CHUNK, left = t.n[k] - base;
-  if (t.dtype[k] == FSGS_DTYPE_F32) chunk_scale((float *)t.g[k] + base, left, c);
-  else if (t.dtype[k] == FSGS_DTYPE_BF16) chunk_scale((__bf16 *)t.g[k] + base, left, c);
-  else chunk_scale((_Float16 *)t.g[k] + base, left, c);
+  turn_of<SCALE_BYTES, true>(t, owner<GRADS>(t.start, t.count, blockIdx.x), blockIdx.x, [&](auto &x) {
+#pragma unroll
+    for (int j = 0; j < (int)(sizeof(x) / sizeof(x[0])); j++) x[j] = (decltype(x[j] + x[j]))((float)x[j] * c);
+  });
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
@@ -626,8 +685,8 @@ int fsgs_adamw_step(int n_tensors, const FsgsAdamWTensor *tensors, int n_hypers,
         }
       }
       const int k = t.count++;
-      t.p[k] = x.param; t.g[k] = x.grad; t.m[k] = x.exp_avg; t.v[k] = x.exp_avg_sq; t.w[k] = x.master;
-      t.scales[k] = x.scales; t.n[k] = x.n; t.start[k] = (uint32_t)groups; t.hyper[k] = (uint8_t)at;
+      t.at[k] = {x.param, x.grad, x.exp_avg, x.exp_avg_sq, x.master, x.scales, x.n, (uint32_t)groups, (uint32_t)at};
+      t.start[k] = (uint32_t)groups;
       groups += chunks_of(x.n);
     }
     if (groups == 0) continue;
@@ -685,9 +744,11 @@ int fsgs_adamw_moments(int n_tensors, const FsgsAdamWMoments *tensors, int write
 }
 
 size_t fsgs_grad_norm_scratch_bytes(int n_tensors) {
-  // a launch takes 48 tensors, or fewer where they hold over 2^35 elements: no card holds 16 times that
-  return n_tensors > 0 ? (size_t)((n_tensors + TENSORS - 1) / TENSORS + 16) * NORM_GROUPS * sizeof(double) : 0;
+  // a launch takes 192 tensors, or fewer where they hold over 2^37 bytes: no card holds that 8 times
+  return n_tensors > 0 ? (size_t)((n_tensors + GRADS - 1) / GRADS + 8) * NORM_GROUPS * sizeof(double) : 0;
 }
+
+static int64_t turns_of(const FsgsGradTensor &g, int bytes) { return (g.n * size_of(g.dtype) + bytes - 1) / bytes; }
 
 static int check_grads(int n_tensors, const FsgsGradTensor *grads, bool write) {
   if (n_tensors < 0 || (n_tensors > 0 && !grads)) return FSGS_ERR_INVALID;
@@ -695,62 +756,78 @@ static int check_grads(int n_tensors, const FsgsGradTensor *grads, bool write) {
   if (!regions.items) return FSGS_ERR_CAPACITY;
   for (int i = 0; i < n_tensors; i++) {
     if (grads[i].n < 0 || !size_of(grads[i].dtype) || (grads[i].n > 0 && !grads[i].grad)) return FSGS_ERR_INVALID;
-    if (chunks_of(grads[i].n) > MAX_BLOCKS) return FSGS_ERR_INVALID;
+    if (grads[i].n > INT64_MAX / 16 || turns_of(grads[i], SCALE_BYTES) > MAX_BLOCKS) return FSGS_ERR_INVALID;
     regions.add(grads[i].grad, grads[i].n * size_of(grads[i].dtype), write);
   }
   return regions.clash() ? FSGS_ERR_INVALID : FSGS_OK;
 }
 
-// the next up to 48 tensors from `from` on that hold at most MAX_BLOCKS chunks; returns the first that is left
-static int fill_grads(GradTable &t, int from, int n_tensors, const FsgsGradTensor *grads) {
+// the next up to 192 tensors from `from` on that make at most MAX_BLOCKS turns; returns the first that is left
+static int fill_grads(GradTable &t, int from, int n_tensors, const FsgsGradTensor *grads, int bytes) {
   std::memset(&t, 0, sizeof(t));
-  int64_t chunks = 0;
+  int64_t turns = 0;
   int i = from;
-  for (; i < n_tensors && i - from < TENSORS; i++) {
+  for (; i < n_tensors && t.count < GRADS; i++) {
     if (grads[i].n == 0) continue;
-    if (chunks + chunks_of(grads[i].n) > MAX_BLOCKS) break;
+    if (turns + turns_of(grads[i], bytes) > MAX_BLOCKS) break;
     const int k = t.count++;
-    t.g[k] = grads[i].grad; t.n[k] = grads[i].n; t.dtype[k] = (uint8_t)grads[i].dtype; t.start[k] = (uint32_t)chunks;
-    chunks += chunks_of(grads[i].n);
+    t.at[k] = {grads[i].grad, grads[i].n << 2 | grads[i].dtype};
+    t.start[k] = (uint32_t)turns;
+    turns += turns_of(grads[i], bytes);
   }
-  t.start[t.count] = (uint32_t)chunks;
+  t.turns = (uint32_t)turns;
   return i;
 }
 
-int fsgs_grad_norm(int n_tensors, const FsgsGradTensor *grads, float max_norm, void *scratch, size_t scratch_bytes,
-                   float *out2, fsgs_stream_t stream_) {
-  hipStream_t stream = (hipStream_t)stream_;
-  if (int rc = check_grads(n_tensors, grads, false)) return rc;
-  if (!out2 || !(max_norm >= 0.0f) || (n_tensors > 0 && !scratch)) return FSGS_ERR_INVALID;
+static int launch_norm(int n_tensors, const FsgsGradTensor *grads, float max_norm, void *scratch, size_t scratch_bytes,
+                       float *norm, float *factor, hipStream_t stream) {
   double *partial = (double *)scratch;
   size_t count = 0;
   GradTable t;
   for (int i = 0; i < n_tensors;) {
-    i = fill_grads(t, i, n_tensors, grads);
+    i = fill_grads(t, i, n_tensors, grads, NORM_BYTES);
     if (t.count == 0) continue;
-    const uint32_t groups = std::min<uint32_t>(t.start[t.count], NORM_GROUPS);
+    const uint32_t groups = std::min<uint32_t>(t.turns, NORM_GROUPS);
     if ((count + groups) * sizeof(double) > scratch_bytes) return FSGS_ERR_CAPACITY;
     hipLaunchKernelGGL(norm_partial_kernel, dim3(groups), dim3(THREADS), 0, stream, t, partial + count);
     FSGS_HIP(hipGetLastError());
     count += groups;
   }
-  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(THREADS), 0, stream, partial, (int)count, max_norm, out2);
+  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(1024), 0, stream, partial, (int)count, max_norm, norm, factor);
   FSGS_HIP(hipGetLastError());
   return FSGS_OK;
 }
 
-int fsgs_grad_scale(int n_tensors, const FsgsGradTensor *grads, const float *coef, fsgs_stream_t stream_) {
-  hipStream_t stream = (hipStream_t)stream_;
-  if (int rc = check_grads(n_tensors, grads, true)) return rc;
-  if (n_tensors > 0 && !coef) return FSGS_ERR_INVALID;
+static int launch_scale(int n_tensors, const FsgsGradTensor *grads, const float *factor, hipStream_t stream) {
   GradTable t;
   for (int i = 0; i < n_tensors;) {
-    i = fill_grads(t, i, n_tensors, grads);
+    i = fill_grads(t, i, n_tensors, grads, SCALE_BYTES);
     if (t.count == 0) continue;
-    hipLaunchKernelGGL(grad_scale_kernel, dim3(t.start[t.count]), dim3(THREADS), 0, stream, t, coef);
+    hipLaunchKernelGGL(grad_scale_kernel, dim3(t.turns), dim3(THREADS), 0, stream, t, factor);
     FSGS_HIP(hipGetLastError());
   }
   return FSGS_OK;
+}
+
+int fsgs_grad_norm(int n_tensors, const FsgsGradTensor *grads, float max_norm, void *scratch, size_t scratch_bytes,
+                   float *norm, float *factor, fsgs_stream_t stream) {
+  if (int rc = check_grads(n_tensors, grads, false)) return rc;
+  if (!norm || !factor || !(max_norm >= 0.0f) || (n_tensors > 0 && !scratch)) return FSGS_ERR_INVALID;
+  return launch_norm(n_tensors, grads, max_norm, scratch, scratch_bytes, norm, factor, (hipStream_t)stream);
+}
+
+int fsgs_grad_scale(int n_tensors, const FsgsGradTensor *grads, const float *factor, fsgs_stream_t stream) {
+  if (int rc = check_grads(n_tensors, grads, true)) return rc;
+  if (n_tensors > 0 && !factor) return FSGS_ERR_INVALID;
+  return launch_scale(n_tensors, grads, factor, (hipStream_t)stream);
+}
+
+int fsgs_grad_clip(int n_tensors, const FsgsGradTensor *grads, float max_norm, void *scratch, size_t scratch_bytes,
+                   float *norm, float *factor, fsgs_stream_t stream) {
+  if (int rc = check_grads(n_tensors, grads, true)) return rc;
+  if (!norm || !factor || !(max_norm >= 0.0f) || (n_tensors > 0 && !scratch)) return FSGS_ERR_INVALID;
+  if (int rc = launch_norm(n_tensors, grads, max_norm, scratch, scratch_bytes, norm, factor, (hipStream_t)stream)) return rc;
+  return launch_scale(n_tensors, grads, factor, (hipStream_t)stream);
 }
 
 }  // extern "C"

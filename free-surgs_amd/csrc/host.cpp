@@ -9,12 +9,13 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty_like.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/DynamicTypes.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
+#include <cstring>
 #include <exception>
 #include <vector>
 
@@ -23,6 +24,7 @@
 namespace {
 
 PyObject *k_step, *k_m, *k_v, *k_mq, *k_vq, *k_scales, *k_master;
+PyObject *k_params, *k_lr, *k_betas, *k_eps, *k_decay, *k_bits, *k_masters, *k_maximize, *k_capturable;
 
 // a plain tensor on the GPU whose elements follow each other in memory
 bool plain(PyObject *o) { return o && THPVariable_CheckExact(o); }
@@ -67,50 +69,76 @@ template <class F> PyObject *guarded(F body) {  // no C++ exception leaves an en
   }
 }
 
-// step_rows(groups, state, bits, masters, dtype) -> (rows, params, states, counts, dtype, others, device index) or None.
-// groups: list of parameter lists, row i of group k has hyper k; counts[k]: steps that group k's tensors have done (-1: no
-// gradient in it).  Of the tensors of `dtype` (-1: that of the first); others: bit c is set where one of type c was passed
-// over.  All on one device.
+struct Bucket {  // tensors of one launch sequence
+  int dtype, bits, device;
+  bool masters, maximize;
+  std::vector<int64_t> rows;
+  std::vector<FsgsAdamWHyper> hypers;
+  PyObject *params, *states;
+};
+struct Buckets : std::vector<Bucket> {
+  ~Buckets() {
+    for (Bucket &b : *this) {
+      Py_XDECREF(b.params);
+      Py_XDECREF(b.states);
+    }
+  }
+};
+
+bool number(PyObject *o, double *x) {  // a float or an int, and nothing that may have a reading of its own
+  if (!o || (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o))) return false;
+  *x = PyFloat_CheckExact(o) ? PyFloat_AS_DOUBLE(o) : PyLong_AsDouble(o);
+  return true;
+}
+bool truth(PyObject *o, bool *x) {
+  if (o != Py_True && o != Py_False) return false;
+  *x = o == Py_True;
+  return true;
+}
+
+// step_rows(param_groups, state) -> [(device index, dtype, bits, maximize, rows, hypers, params, states)] or None
 PyObject *step_rows(PyObject *, PyObject *args) {
   PyObject *groups, *state;
-  int bits, masters, want;
-  if (!PyArg_ParseTuple(args, "O!O!iii", &PyList_Type, &groups, &PyDict_Type, &state, &bits, &masters, &want)) return nullptr;
+  if (!PyArg_ParseTuple(args, "O!O!", &PyList_Type, &groups, &PyDict_Type, &state)) return nullptr;
   return guarded([&]() -> PyObject * {
-    Ref params(PyList_New(0)), states(PyList_New(0)), counts(PyList_New(0));
-    if (!params.o || !states.o || !counts.o) return nullptr;
-    std::vector<int64_t> rows;
-    PyObject *const km = bits == 8 ? k_mq : k_m, *const kv = bits == 8 ? k_vq : k_v;
-    const at::ScalarType moment = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
-    c10::Device device(c10::kCPU);
-    int others = 0;
+    Buckets buckets;
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(groups); k++) {
       PyObject *group = PyList_GET_ITEM(groups, k);
-      if (!PyList_Check(group)) return other_case();
-      long long count = -1;
-      for (Py_ssize_t i = 0; i < PyList_GET_SIZE(group); i++) {
-        PyObject *o = PyList_GET_ITEM(group, i);
+      if (!PyDict_Check(group)) return other_case();
+      PyObject *betas = PyDict_GetItemWithError(group, k_betas), *list = PyDict_GetItemWithError(group, k_params);
+      FsgsAdamWHyper h = {};
+      double bits;
+      bool masters, maximize, capturable;
+      if (!betas || !PyTuple_CheckExact(betas) || PyTuple_GET_SIZE(betas) != 2 || !list || !PyList_Check(list) ||
+          !number(PyDict_GetItemWithError(group, k_lr), &h.lr) || !number(PyTuple_GET_ITEM(betas, 0), &h.beta1) ||
+          !number(PyTuple_GET_ITEM(betas, 1), &h.beta2) || !number(PyDict_GetItemWithError(group, k_eps), &h.eps) ||
+          !number(PyDict_GetItemWithError(group, k_decay), &h.weight_decay) ||
+          !number(PyDict_GetItemWithError(group, k_bits), &bits) || (bits != 8 && bits != 32) ||
+          !truth(PyDict_GetItemWithError(group, k_masters), &masters) ||
+          !truth(PyDict_GetItemWithError(group, k_maximize), &maximize) ||
+          !truth(PyDict_GetItemWithError(group, k_capturable), &capturable) || capturable)
+        return other_case();
+      if (!(h.lr >= 0.0 && h.beta1 >= 0.0 && h.beta1 < 1.0 && h.beta2 >= 0.0 && h.beta2 < 1.0 && h.eps >= 0.0 && h.weight_decay >= 0.0))
+        return other_case();
+      PyObject *const km = bits == 8 ? k_mq : k_m, *const kv = bits == 8 ? k_vq : k_v;
+      const at::ScalarType moment = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
+      for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); i++) {
+        PyObject *o = PyList_GET_ITEM(list, i);
         if (!plain(o)) return other_case();
         const at::Tensor &p = THPVariable_Unpack(o);
         const at::Tensor &g = p.grad();
         if (!g.defined()) continue;
         const at::ScalarType type = p.scalar_type();
-        const int code = dtype_code(type);
-        if (code < 0) return other_case();
-        if (want < 0) want = code;
-        if (want != code) {
-          others |= 1 << code;
-          continue;
-        }
-        if (rows.empty()) device = p.device();
+        const c10::Device device = p.device();
         const int64_t n = p.numel();
-        if (!fits(p, type, device, n) || !fits(g, type, device, n)) return other_case();
+        const int code = dtype_code(type);
+        if (code < 0 || !packed(p) || !fits(g, type, device, n)) return other_case();
         PyObject *st = PyDict_GetItemWithError(state, o);
         if (!st || !PyDict_Check(st)) return other_case();
         PyObject *step = PyDict_GetItemWithError(st, k_step);
         if (!step || !PyLong_CheckExact(step)) return other_case();
-        const long long done = PyLong_AsLongLong(step);
-        if (done < 0 || (count >= 0 && done != count)) return other_case();
-        count = done;
+        h.step = PyLong_AsLongLong(step) + 1;
+        if (h.step < 1) return other_case();
         const at::Tensor *m = entry(st, km), *v = m ? entry(st, kv) : nullptr, *s = nullptr, *w = nullptr;
         if (!m || !v || !fits(*m, moment, device, n) || !fits(*v, moment, device, n)) return other_case();
         if (bits == 8) {
@@ -121,18 +149,35 @@ PyObject *step_rows(PyObject *, PyObject *args) {
           w = entry(st, k_master);
           if (!w || !fits(*w, at::kFloat, device, n)) return other_case();
         }
-        if (PyList_Append(params.o, o) || PyList_Append(states.o, st)) return nullptr;
-        const int64_t row[] = {address(p), address(g), address(*m), address(*v), s ? address(*s) : 0, w ? address(*w) : 0, n, k};
+        Bucket *b = nullptr;
+        for (Bucket &x : buckets)
+          if (x.dtype == code && x.bits == (int)bits && x.device == device.index() && x.masters == (w != nullptr) && x.maximize == maximize)
+            b = &x;
+        if (!b) {
+          buckets.push_back({code, (int)bits, device.index(), w != nullptr, maximize, {}, {}, PyList_New(0), PyList_New(0)});
+          b = &buckets.back();
+          if (!b->params || !b->states) return nullptr;
+        }
+        // most tensors share the scalars of the one in front of them; other repetitions cost a place in the list
+        if (b->hypers.empty() || std::memcmp(&b->hypers.back(), &h, sizeof(h))) b->hypers.push_back(h);
+        if (PyList_Append(b->params, o) || PyList_Append(b->states, st)) return nullptr;
+        const int64_t row[] = {address(p), address(g), address(*m), address(*v), s ? address(*s) : 0, w ? address(*w) : 0, n,
+                               (int64_t)b->hypers.size() - 1};
         static_assert(sizeof(row) == sizeof(FsgsAdamWTensor), "a row");
-        rows.insert(rows.end(), row, row + 8);
+        b->rows.insert(b->rows.end(), row, row + 8);
       }
-      Ref c(PyLong_FromLongLong(count));
-      if (!c.o || PyList_Append(counts.o, c.o)) return nullptr;
     }
-    Ref bytes(rows_of(rows));
-    if (!bytes.o) return nullptr;
-    return Py_BuildValue("(OOOOiii)", bytes.o, params.o, states.o, counts.o, want, others,
-                         rows.empty() ? -1 : (int)device.index());
+    Ref out(PyList_New(0));
+    if (!out.o) return nullptr;
+    for (const Bucket &b : buckets) {
+      Ref rows(rows_of(b.rows));
+      Ref hypers(PyBytes_FromStringAndSize((const char *)b.hypers.data(), (Py_ssize_t)(b.hypers.size() * sizeof(FsgsAdamWHyper))));
+      if (!rows.o || !hypers.o) return nullptr;
+      Ref item(Py_BuildValue("(iiiOOOOO)", b.device, b.dtype, b.bits, b.maximize ? Py_True : Py_False, rows.o, hypers.o, b.params,
+                             b.states));
+      if (!item.o || PyList_Append(out.o, item.o)) return nullptr;
+    }
+    return out.release();
   });
 }
 
@@ -193,36 +238,54 @@ PyObject *grads_written(PyObject *, PyObject *params) {
   });
 }
 
-// moment_rows(states, dtype) -> ([(m, v)], rows, device index) for states whose moments are in 8 bits, or None: new tensors
-// of `dtype` for the values
+// moment_rows(param_groups, state, dtype) -> ([(m, v)], rows, device index) of the parameters that have a state, in order, or None:
+// new tensors of `dtype` for the values of 8-bit moments
 PyObject *moment_rows(PyObject *, PyObject *args) {
-  PyObject *states, *dtype;
-  if (!PyArg_ParseTuple(args, "O!O", &PyList_Type, &states, &dtype)) return nullptr;
+  PyObject *groups, *state, *dtype;
+  if (!PyArg_ParseTuple(args, "O!O!O", &PyList_Type, &groups, &PyDict_Type, &state, &dtype)) return nullptr;
   if (!THPDtype_Check(dtype)) { PyErr_SetString(PyExc_TypeError, "a dtype"); return nullptr; }
   return guarded([&]() -> PyObject * {
     const at::ScalarType type = ((THPDtype *)dtype)->scalar_type;
-    std::vector<int64_t> rows;
-    Ref pairs(PyList_New(0));
-    if (!pairs.o) return nullptr;
+    struct Item { const at::Tensor *m, *v, *s; };
+    std::vector<Item> items;
     c10::Device device(c10::kCPU);
-    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(states); i++) {
-      PyObject *st = PyList_GET_ITEM(states, i);
-      if (!PyDict_Check(st)) return other_case();
-      const at::Tensor *mq = entry(st, k_mq), *vq = mq ? entry(st, k_vq) : nullptr, *s = vq ? entry(st, k_scales) : nullptr;
-      if (!s) return other_case();
-      const int64_t n = mq->numel();
-      if (i == 0) device = mq->device();
-      if (!fits(*mq, at::kFloat8_e4m3fn, device, n) || !fits(*vq, at::kFloat8_e4m3fn, device, n) ||
-          !fits(*s, at::kByte, device, 2 * ((n + FSGS_ADAMW_BLOCK - 1) / FSGS_ADAMW_BLOCK)))
-        return other_case();
-      const at::Tensor m = at::empty_like(*mq, mq->options().dtype(type)), v = at::empty_like(*mq, mq->options().dtype(type));
-      const int64_t row[] = {address(*mq), address(*vq), address(*s), address(m), address(v), n};
+    for (Py_ssize_t k = 0; k < PyList_GET_SIZE(groups); k++) {
+      PyObject *group = PyList_GET_ITEM(groups, k), *list = PyDict_Check(group) ? PyDict_GetItemWithError(group, k_params) : nullptr;
+      if (!list || !PyList_Check(list)) return other_case();
+      for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); i++) {
+        PyObject *o = PyList_GET_ITEM(list, i), *st = PyDict_GetItemWithError(state, o);
+        if (PyErr_Occurred()) return nullptr;
+        if (!st) continue;
+        if (!plain(o) || !PyDict_Check(st)) return other_case();
+        const int64_t n = THPVariable_Unpack(o).numel();
+        const at::Tensor *mq = entry(st, k_mq), *vq = mq ? entry(st, k_vq) : nullptr, *s = vq ? entry(st, k_scales) : nullptr;
+        if (!s) return other_case();
+        if (items.empty()) device = mq->device();
+        if (!fits(*mq, at::kFloat8_e4m3fn, device, n) || !fits(*vq, at::kFloat8_e4m3fn, device, n) ||
+            mq->sizes() != THPVariable_Unpack(o).sizes() ||
+            !fits(*s, at::kByte, device, 2 * ((n + FSGS_ADAMW_BLOCK - 1) / FSGS_ADAMW_BLOCK)))
+          return other_case();
+        items.push_back({mq, vq, s});
+      }
+    }
+    if (items.empty()) return other_case();
+    Ref pairs(PyList_New((Py_ssize_t)items.size()));
+    if (!pairs.o) return nullptr;
+    std::vector<int64_t> rows;
+    rows.reserve(6 * items.size());
+    for (size_t i = 0; i < items.size(); i++) {
+      const Item &x = items[i];
+      // torch's own function behind torch.empty, without an operator's dispatch for each of what may be hundreds
+      const at::Tensor m(at::detail::empty_cuda(x.m->sizes(), type, device, std::nullopt)),
+          v(at::detail::empty_cuda(x.m->sizes(), type, device, std::nullopt));
+      const int64_t row[] = {address(*x.m), address(*x.v), address(*x.s), address(m), address(v), x.m->numel()};
       static_assert(sizeof(row) == sizeof(FsgsAdamWMoments), "a row");
       rows.insert(rows.end(), row, row + 6);
       Ref a(THPVariable_Wrap(m)), b(THPVariable_Wrap(v));
       if (!a.o || !b.o) return nullptr;
-      Ref pair(PyTuple_Pack(2, a.o, b.o));
-      if (!pair.o || PyList_Append(pairs.o, pair.o)) return nullptr;
+      PyObject *pair = PyTuple_Pack(2, a.o, b.o);
+      if (!pair) return nullptr;
+      PyList_SET_ITEM(pairs.o, (Py_ssize_t)i, pair);
     }
     Ref bytes(rows_of(rows));
     if (!bytes.o) return nullptr;
@@ -231,11 +294,11 @@ PyObject *moment_rows(PyObject *, PyObject *args) {
 }
 
 PyMethodDef methods[] = {
-    {"step_rows", step_rows, METH_VARARGS, "(rows, params, states, counts, dtype, others, device) of an ordinary step, or None"},
+    {"step_rows", step_rows, METH_VARARGS, "the launch sequences of an ordinary step, or None"},
     {"stepped", stepped, METH_VARARGS, "count a step in every state and raise the parameters' versions"},
     {"grad_rows", grad_rows, METH_O, "(rows, device) of the parameters' gradients, or None"},
     {"grads_written", grads_written, METH_O, "raise the versions of the parameters' gradients"},
-    {"moment_rows", moment_rows, METH_VARARGS, "(pairs, rows, device) of 8-bit moments, or None"},
+    {"moment_rows", moment_rows, METH_VARARGS, "(pairs, rows, device) of the 8-bit moments of all parameters, or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fsgs_host", "the optimiser's walk over its tensors", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
@@ -245,7 +308,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fsgs_host", "the optimiser's walk
 PyMODINIT_FUNC PyInit__fsgs_host(void) {
   struct { PyObject **key; const char *name; } keys[] = {
       {&k_step, "step"}, {&k_m, "exp_avg"}, {&k_v, "exp_avg_sq"}, {&k_mq, "exp_avg_q"},
-      {&k_vq, "exp_avg_sq_q"}, {&k_scales, "scales"}, {&k_master, "master"}};
+      {&k_vq, "exp_avg_sq_q"}, {&k_scales, "scales"}, {&k_master, "master"}, {&k_params, "params"},
+      {&k_lr, "lr"}, {&k_betas, "betas"}, {&k_eps, "eps"}, {&k_decay, "weight_decay"}, {&k_bits, "state_bits"},
+      {&k_masters, "master_weights"}, {&k_maximize, "maximize"}, {&k_capturable, "capturable"}};
   for (auto &k : keys)
     if (!(*k.key = PyUnicode_InternFromString(k.name))) return nullptr;
   return PyModule_Create(&module);

@@ -83,7 +83,7 @@ class FsgsAdamGroup(C.Structure):
 # FsgsAdamWTensor / FsgsAdamWMoments / FsgsGradTensor are rows of 64-bit words (include/fsgs.h): the optimiser fills them as flat
 # array('q') buffers, several times faster than ctypes fields over hundreds of tensors
 ADAMW_TENSOR_WORDS, ADAMW_MOMENTS_WORDS, GRAD_TENSOR_WORDS = 8, 6, 3
-ADAMW_BLOCK = 128
+ADAMW_BLOCK, ADAMW_HYPER_BYTES = 128, 64
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 
 
@@ -201,7 +201,8 @@ _PROTOTYPES = {
     "fsgs_adamw_step": (_i, [_i, _vp, _i, _vp, _i, _i, _i, _vp, _vp, _vp]),
     "fsgs_adamw_moments": (_i, [_i, _vp, _i, _i, _vp]),
     "fsgs_grad_norm_scratch_bytes": (_sz, [_i]),
-    "fsgs_grad_norm": (_i, [_i, _vp, C.c_float, _vp, _sz, _vp, _vp]),
+    "fsgs_grad_norm": (_i, [_i, _vp, C.c_float, _vp, _sz, _vp, _vp, _vp]),
+    "fsgs_grad_clip": (_i, [_i, _vp, C.c_float, _vp, _sz, _vp, _vp, _vp]),
     "fsgs_grad_scale": (_i, [_i, _vp, _vp, _vp]),
     "fsgs_densify_plan": (_i, [_i, _vp, _vp, _vp, _vp, C.c_float, C.c_float, C.c_float, C.c_float, _i, _vp, _vp]),
     "fsgs_densify_apply": (_i, [_i, _vp, _vp, C.POINTER(C.c_int32), _i, C.POINTER(FsgsDensifyGroup), _vp, _vp, _vp,

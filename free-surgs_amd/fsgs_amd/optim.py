@@ -106,36 +106,36 @@ def _check_grad(g, name="gradient"):
         raise TypeError("%s: float32, bfloat16 or float16, got %s" % (name, g.dtype))
 
 
-def _norm_of(lib, dev, table, max_norm):
-    """float32 [2] = {norm, factor} of the gradients in a table (rows of FsgsGradTensor), on dev's current stream"""
-    n = len(table) // _lib.GRAD_TENSOR_WORDS
-    nbytes = lib.fsgs_grad_norm_scratch_bytes(n)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    out = torch.empty(2, dtype=_F32, device=dev)
-    _lib.check(lib.fsgs_grad_norm(n, _address(table), max_norm, scratch.data_ptr(), nbytes, out.data_ptr(),
-                                  _lib.current_stream()), "fsgs_grad_norm")
-    return out
+def _norm_of(entry, dev, table, max_norm):
+    """(return code, norm, tensor whose first float is the factor) of fsgs_grad_norm / _clip on the gradients in a table
+    (rows of FsgsGradTensor, as bytes), on dev's current stream"""
+    n = len(table) // (8 * _lib.GRAD_TENSOR_WORDS)
+    nbytes = _lib.load().fsgs_grad_norm_scratch_bytes(n)
+    norm = torch.empty((), dtype=_F32, device=dev)
+    scratch = torch.empty(16 + nbytes, dtype=torch.uint8, device=dev)
+    factor = scratch.data_ptr()
+    return entry(n, table, max_norm, factor + 16, nbytes, norm.data_ptr(), factor, _lib.current_stream()), norm, scratch
 
 
-def _grad_table(params, grads, who):
-    """(device, rows, what to keep until the launch, gradients that are not dense) of the gradients of params"""
+def _grad_table(params, who):
+    """(device, rows, whether all are packed, what to keep until the launch) of the gradients of params; the device is None
+    where there are none"""
     fast = _lib.host().grad_rows(params)
     if fast is not None:
-        return torch.device("cuda", fast[1]), array("q", fast[0]), None, []
-    return _table_of(grads, who)
+        return (torch.device("cuda", fast[1]) if fast[1] >= 0 else None), fast[0], True, None
+    return _table_of([p.grad for p in params if p.grad is not None], who)
 
 
 def _table_of(grads, who):
-    dev, table, keep, strided = _one_device(grads, who), array("q"), [], []
+    dev, table, keep, dense = _one_device(grads, who), array("q"), [], True
     for g in grads:
         if g.is_neg():
             raise RuntimeError("%s: a gradient is a negated view (resolve_neg)" % who)
         if not _dense(g):
-            strided.append(g)
-            g = g.contiguous()
+            dense, g = False, g.contiguous()
             keep.append(g)
         table.extend((g.data_ptr(), g.numel(), _DTYPES[g.dtype]))
-    return dev, table, keep, strided
+    return dev, table.tobytes(), dense, keep
 
 
 def _one_device(grads, who):
@@ -162,45 +162,42 @@ def grad_norm(tensors):
     if not tensors:
         return torch.tensor(0.0)
     lib = _lib.load()
-    dev, table, _keep, _ = _table_of(tensors, "grad_norm")
+    dev, table, _, _keep = _table_of(tensors, "grad_norm")
     with _on(dev):
-        return _norm_of(lib, dev, table, float("inf"))[0]
+        rc, norm, _ = _norm_of(lib.fsgs_grad_norm, dev, table, float("inf"))
+    _lib.check(rc, "fsgs_grad_norm")
+    return norm
 
 
 @torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
-    """torch.nn.utils.clip_grad_norm_ in three launches per 48 tensors: the gradients' global 2-norm, and every gradient
-    scaled in place by min(1, max_norm / (norm + 1e-6)); where that factor is 1 no gradient is read again.  Returns the norm
-    (0-d float32) without a host synchronisation, unless error_if_nonfinite asks for one."""
+    """torch.nn.utils.clip_grad_norm_ in three launches per 192 tensors: the gradients' global 2-norm, and every gradient
+    (dense, on one device, float32 / bfloat16 / float16 side by side) scaled in place by min(1, max_norm / (norm + 1e-6));
+    where that factor is 1 no gradient is read again.  Returns the norm (0-d float32) without a host synchronisation, unless
+    error_if_nonfinite asks for one."""
     if float(norm_type) != 2.0:
         raise ValueError("clip_grad_norm_: the 2-norm only, got norm_type=%r" % (norm_type,))
     max_norm = _max_norm(max_norm)
     parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
-    grads = [p.grad for p in parameters if p.grad is not None]
-    if not grads:
-        return torch.tensor(0.0)
     lib = _lib.load()
-    dev, table, _keep, strided = _grad_table(parameters, grads, "clip_grad_norm_")
-    scaled = table
-    if strided:
-        if len({id(g) for g in grads}) != len(grads):
-            raise ValueError("clip_grad_norm_: a parameter is given twice")
-        scaled = _table_of([g for g in grads if _dense(g)], "clip_grad_norm_")[1] if len(strided) < len(grads) else array("q")
+    dev, table, dense, slow = _grad_table(parameters, "clip_grad_norm_")
+    if dev is None:
+        return torch.tensor(0.0)
+    if not dense:
+        raise ValueError("clip_grad_norm_: gradients are dense in memory; scale slices of other tensors by hand")
     with _on(dev):
-        out = _norm_of(lib, dev, table, max_norm)
-        norm, coef = out[0], out[1]
-        if error_if_nonfinite and not bool(torch.isfinite(norm)):
-            raise RuntimeError("clip_grad_norm_: the gradients' norm is %s" % float(norm))
-        rc = lib.fsgs_grad_scale(len(scaled) // _lib.GRAD_TENSOR_WORDS, _address(scaled), out.data_ptr() + 4, _lib.current_stream())
+        rc, norm, factor = _norm_of(lib.fsgs_grad_norm if error_if_nonfinite else lib.fsgs_grad_clip, dev, table, max_norm)
+        if error_if_nonfinite and rc == _lib.FSGS_OK:
+            if not bool(torch.isfinite(norm)):
+                raise RuntimeError("clip_grad_norm_: the gradients' norm is %s" % float(norm))
+            rc = lib.fsgs_grad_scale(len(table) // (8 * _lib.GRAD_TENSOR_WORDS), table, factor.data_ptr(), _lib.current_stream())
         if rc == _lib.FSGS_ERR_INVALID:
             raise ValueError("clip_grad_norm_: two of the gradients share memory, or a parameter is given twice")
-        _lib.check(rc, "fsgs_grad_scale")
-        for g in strided:  # slices of other tensors; expanded ones torch itself refuses to write
-            g.copy_(g.float() * coef)
-        if strided or _keep is not None:
-            mark_updated(grads)
-        else:
-            _lib.host().grads_written(parameters)
+        _lib.check(rc, "fsgs_grad_clip")
+    if slow is None:
+        _lib.host().grads_written(parameters)
+    else:
+        mark_updated([p.grad for p in parameters if p.grad is not None])
     return norm
 
 
@@ -327,11 +324,6 @@ class FusedAdamW(torch.optim.Optimizer):
     def _read(self, items, dtype):
         """values of 8-bit moments: one launch per 48 tensors of a device"""
         lib, out, by_device = _lib.load(), [], {}
-        fast = _lib.host().moment_rows([st for _, st in items], dtype) if items else None
-        if fast is not None and all(st["exp_avg_q"].shape == p.shape for p, st in items):
-            out, rows, index = fast
-            by_device[torch.device("cuda", index)] = array("q", rows)
-            items = ()
         for p, st in items:
             mq, vq, scales = self._state_tensors(p, st, 8)
             if not p.is_cuda:
@@ -366,6 +358,13 @@ class FusedAdamW(torch.optim.Optimizer):
         `dtype`.  float32 and bfloat16 hold what 8-bit moments stand for exactly."""
         if dtype not in _DTYPES:
             raise TypeError("moments: float32, bfloat16 or float16, got %s" % dtype)
+        fast = _lib.host().moment_rows(self.param_groups, self.state, dtype)
+        if fast is not None:  # all of them in 8 bits, packed, on one device
+            pairs, rows, index = fast
+            with _on(torch.device("cuda", index)):
+                _lib.check(_lib.load().fsgs_adamw_moments(len(pairs), rows, 0, _DTYPES[dtype], _lib.current_stream()),
+                           "fsgs_adamw_moments")
+            return pairs
         items = [(p, self.state[p]) for group in self.param_groups for p in group["params"]
                  if p in self.state and ("exp_avg" in self.state[p] or "exp_avg_q" in self.state[p])]
         read = iter(self._read([it for it in items if "exp_avg_q" in it[1]], dtype))
@@ -437,17 +436,19 @@ class FusedAdamW(torch.optim.Optimizer):
             return loss
         coef = None
         if self.max_grad_norm is not None:
-            params = [p for bucket in work for p in bucket.params]
-            dev, table, _keep, _ = _grad_table(params, [p.grad for p in params], "FusedAdamW(max_grad_norm)")
+            params = work[0].params if len(work) == 1 else [p for bucket in work for p in bucket.params]
+            dev, table, _, _keep = _grad_table(params, "FusedAdamW(max_grad_norm)")
             with _on(dev):
-                out = _norm_of(lib, dev, table, self.max_grad_norm)
-            self.last_grad_norm, coef = out[0], out.data_ptr() + 4
+                rc, self.last_grad_norm, factor = _norm_of(lib.fsgs_grad_norm, dev, table, self.max_grad_norm)
+            _lib.check(rc, "fsgs_grad_norm")
+            coef = factor.data_ptr()
         for b in work:
-            n = len(b.table) // _lib.ADAMW_TENSOR_WORDS
+            n = len(b.params)
+            rows, hypers = b.arrays()
             with _on(b.device):
                 scratch = torch.empty(lib.fsgs_adamw_scratch_bytes(n), dtype=torch.uint8, device=b.device) if b.capturable else None
-                rc = lib.fsgs_adamw_step(n, _address(b.table), len(b.hypers), (_lib.FsgsAdamWHyper * len(b.hypers))(*b.hypers),
-                                         b.dtype, b.bits, b.maximize, coef, _lib.ptr(scratch), _lib.current_stream())
+                rc = lib.fsgs_adamw_step(n, rows, len(hypers) // _lib.ADAMW_HYPER_BYTES, hypers, b.dtype, b.bits, b.maximize, coef,
+                                         _lib.ptr(scratch), _lib.current_stream())
                 if rc == _lib.FSGS_ERR_INVALID:
                     raise ValueError("FusedAdamW: two of the tensors of a step share memory")
                 _lib.check(rc, "fsgs_adamw_step")
@@ -455,33 +456,15 @@ class FusedAdamW(torch.optim.Optimizer):
         return loss
 
     def _ordinary(self):
-        """The buckets of a step whose tensors are all as one expects them -- packed, on one device, with their states in
-        place and counted alike within a group -- collected by the host extension; None where anything is not."""
-        by_key = {}
-        for group in self.param_groups:
-            if group["capturable"]:
-                return None
-            key = (group["state_bits"], bool(group["master_weights"]), bool(group["maximize"]))
-            lists, scalars = by_key.setdefault(key, ([], []))
-            lists.append(group["params"])
-            scalars.append(self._scalars(group)[:5])
+        """The buckets of a step whose tensors and options are all as one expects them -- packed tensors with their states in
+        place, options that are plain numbers in range -- collected by the host extension; None where anything is not."""
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             return None
-        work, rows = [], _lib.host().step_rows
-        for (bits, masters, maximize), (lists, scalars) in by_key.items():
-            types = [-1]  # the first tensor's, then what else there is
-            for dtype in types:
-                found = rows(lists, self.state, bits, masters, dtype)
-                if found is None:
-                    return None
-                table, params, states, counts, code, others, index = found
-                if dtype < 0:
-                    types += [c for c in _DTYPES.values() if others >> c & 1]
-                if params:
-                    hypers = [(*h, c + 1 if c >= 0 else 1, None, None) for h, c in zip(scalars, counts)]
-                    work.append(_Bucket(torch.device("cuda", index), code, bits, maximize, False, array("q", table), hypers, params,
-                                        states))
-        return work
+        found = _lib.host().step_rows(self.param_groups, self.state)
+        if found is None:
+            return None
+        return [_Bucket(torch.device("cuda", index), dtype, bits, maximize, False, rows, hypers, params, states)
+                for index, dtype, bits, maximize, rows, hypers, params, states in found]
 
     def _general(self):
         """The buckets of any step that can be made: every tensor looked at in turn; states made or converted."""
@@ -556,6 +539,12 @@ class _Bucket:
         self.device, self.dtype, self.bits, self.maximize, self.capturable = device, dtype, bits, maximize, capturable
         self.table, self.hypers, self.params, self.states = table, hypers, params, states
         self.index, self.keep = {}, []
+
+    def arrays(self):
+        """(tensors, hypers) as the bytes that the C entry reads"""
+        if isinstance(self.table, bytes):
+            return self.table, self.hypers
+        return self.table.tobytes(), bytes((_lib.FsgsAdamWHyper * len(self.hypers))(*self.hypers))
 
 
 def densify_stats(radii, viewspace_grad, max_radii2D, xyz_gradient_accum, denom):

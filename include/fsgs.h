@@ -544,7 +544,7 @@ typedef struct FsgsAdamWHyper {
 } FsgsAdamWHyper;
 /* bytes of the scratch that a call with step_dev needs (kept until its kernels have run) */
 size_t fsgs_adamw_scratch_bytes(int n_tensors);
-/* tensors, hypers: HOST arrays.  grad_coef: float[1] DEVICE factor on the gradients (out2 + 1 of fsgs_grad_norm) or NULL.
+/* tensors, hypers: HOST arrays.  grad_coef: float[1] DEVICE factor on the gradients (`factor` of fsgs_grad_norm) or NULL.
  * scratch: NULL without step_dev. */
 int fsgs_adamw_step(int n_tensors, const FsgsAdamWTensor *tensors, int n_hypers, const FsgsAdamWHyper *hypers, int dtype,
                     int state_bits, int maximize, const float *grad_coef, void *scratch, fsgs_stream_t stream);
@@ -560,9 +560,9 @@ typedef struct FsgsAdamWMoments {
 } FsgsAdamWMoments;
 int fsgs_adamw_moments(int n_tensors, const FsgsAdamWMoments *tensors, int write, int dtype, fsgs_stream_t stream);
 
-/* Global 2-norm of any number of gradients (squares summed in 64 bits, in a fixed order) and what bounds it:
- * out2 float[2] DEVICE = {norm, min(1, max_norm / (norm + 1e-6))}; a NaN norm gives a NaN factor.  The same memory may
- * be given twice (and counts twice).  scratch: fsgs_grad_norm_scratch_bytes(n_tensors), need not be cleared. */
+/* Global 2-norm of any number of gradients (squares summed in 64 bits, in a fixed order) and what bounds it, both float[1] on
+ * the DEVICE: norm, and factor = min(1, max_norm / (norm + 1e-6)); a NaN norm gives a NaN factor.  The same memory may be
+ * given twice (and counts twice).  scratch: fsgs_grad_norm_scratch_bytes(n_tensors), need not be cleared. */
 typedef struct FsgsGradTensor {
   void *grad;
   int64_t n;
@@ -571,9 +571,13 @@ typedef struct FsgsGradTensor {
 } FsgsGradTensor;
 size_t fsgs_grad_norm_scratch_bytes(int n_tensors);
 int fsgs_grad_norm(int n_tensors, const FsgsGradTensor *grads, float max_norm, void *scratch, size_t scratch_bytes,
-                   float *out2, fsgs_stream_t stream);
-/* grad *= coef[0] (DEVICE) in place, rounded to the gradient's type; a factor of exactly 1 moves no data. */
-int fsgs_grad_scale(int n_tensors, const FsgsGradTensor *grads, const float *coef, fsgs_stream_t stream);
+                   float *norm, float *factor, fsgs_stream_t stream);
+/* grad *= factor[0] (DEVICE) in place, rounded to the gradient's type; a factor of exactly 1 moves no data.  No two may
+ * share memory. */
+int fsgs_grad_scale(int n_tensors, const FsgsGradTensor *grads, const float *factor, fsgs_stream_t stream);
+/* both */
+int fsgs_grad_clip(int n_tensors, const FsgsGradTensor *grads, float max_norm, void *scratch, size_t scratch_bytes,
+                   float *norm, float *factor, fsgs_stream_t stream);
 
 /* For every Gaussian with radii > 0: max_radii2D = max(., radii); xyz_gradient_accum += ||viewspace_grad||;
  * denom += 1   (scene/gaussian_model.py:678-681, train.py:298-303).  viewspace_grad [P,3]. */

@@ -87,13 +87,15 @@ def test_moments_norm_and_scale_refuse():
 
     def norm(r, bound=1.0, out=A, scratch=A, nbytes=1 << 20):
         table = array("q", r)
-        return lib.fsgs_grad_norm(1, table.buffer_info()[0], bound, scratch, nbytes, out, None)
+        return lib.fsgs_grad_norm(1, table.buffer_info()[0], bound, scratch, nbytes, out, A + 128, None)
 
     assert norm((A, -1, 0)) == norm((0, 4, 0)) == norm((A, 4, 9)) == norm((A, 1 << 50, 0)) == INVALID
     assert norm((A, 4, 0), -1.0) == norm((A, 4, 0), float("nan")) == norm((A, 4, 0), out=None) == norm((A, 4, 0), scratch=None) == INVALID
     assert norm((A, 4, 0), nbytes=0) == _lib.FSGS_ERR_CAPACITY
     twice = array("q", (A, 4, 0, A + 12, 4, 0))
     assert lib.fsgs_grad_scale(2, twice.buffer_info()[0], A + 64, None) == INVALID
+    assert lib.fsgs_grad_clip(2, twice.buffer_info()[0], 1.0, A, 1 << 20, A + 64, A + 128, None) == INVALID
+    assert lib.fsgs_grad_clip(1, twice.buffer_info()[0], 1.0, A, 1 << 20, A + 64, None, None) == INVALID
     assert lib.fsgs_grad_scale(1, twice.buffer_info()[0], None, None) == INVALID
     assert lib.fsgs_grad_scale(0, None, None, None) == 0
 

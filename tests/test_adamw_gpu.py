@@ -479,9 +479,18 @@ def test_norm_of_mixed_types_large_values_and_nan():
         clip_grad_norm_([q, r], 0.1)
     assert bool((q.grad == 1).all())
     s = torch.ones(6, device=DEV, requires_grad=True)
-    s.grad = torch.full((6, 2), 2.0, device=DEV)[:, 0]            # strided
-    assert abs(float(clip_grad_norm_([s], 1.0)) - math.sqrt(24)) < 1e-5
-    assert float((s.grad - 2 / math.sqrt(24)).abs().max()) < 1e-6
+    s.grad = torch.full((6, 2), 2.0, device=DEV)[:, 0]            # a slice
+    assert abs(float(grad_norm(s.grad)) - math.sqrt(24)) < 1e-5
+    with pytest.raises(ValueError, match="dense"):
+        clip_grad_norm_([q, s], 1.0)
+    assert bool((q.grad == 1).all())
+    a, b = torch.ones(4, 5, device=DEV).t().requires_grad_(True), torch.ones(3, device=DEV, dtype=torch.float16, requires_grad=True)
+    a.grad, b.grad = torch.full((4, 5), 3.0, device=DEV).t(), torch.full((3,), 2.0, device=DEV, dtype=torch.float16)
+    for error in (True, False):  # a gradient of another order of dimensions, types side by side; both ways through
+        want = math.sqrt(float((a.grad.double() ** 2).sum() + (b.grad.double() ** 2).sum()))
+        g = a.grad.clone()
+        assert abs(float(clip_grad_norm_([a, b], want / 2, error_if_nonfinite=error)) - want) <= 2 * E32 * want
+        assert float((a.grad - g / 2).abs().max()) < 1e-6
 
 
 def test_the_norm_bound_inside_a_step_is_the_clip_in_front_of_it():
