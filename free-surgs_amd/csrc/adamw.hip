@@ -49,7 +49,7 @@ constexpr int CHUNK = 2048;
 // Bytes of one workgroup's turn: four 16-byte vectors a thread in the norm, two in the scaling (160 bf16 layers of 64 M: norm
 // 27.6 us, with two 30.9, with eight 28.5; scaling 48.0 us, with four 51.7, with one 60.1).
 constexpr int NORM_BYTES = 16384, SCALE_BYTES = 8192;
-constexpr int64_t MAX_BLOCKS = 1 << 23;  // workgroups of one launch (256 threads each: 2^31 work items)
+constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;  // workgroups of one launch (256 threads each: under 2^32 work items)
 constexpr int QBLOCK = FSGS_ADAMW_BLOCK;  // elements that share a power of two
 constexpr int NORM_GROUPS = 2048;      // workgroups of one norm launch at most: eight per CU
 
@@ -744,7 +744,7 @@ int fsgs_adamw_moments(int n_tensors, const FsgsAdamWMoments *tensors, int write
 }
 
 size_t fsgs_grad_norm_scratch_bytes(int n_tensors) {
-  // a launch takes 192 tensors, or fewer where they hold over 2^37 bytes: no card holds that 8 times
+  // a launch takes 192 tensors, or fewer where they hold over 2^38 bytes: no card holds that 8 times
   return n_tensors > 0 ? (size_t)((n_tensors + GRADS - 1) / GRADS + 8) * NORM_GROUPS * sizeof(double) : 0;
 }
 

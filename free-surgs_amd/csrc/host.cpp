@@ -148,6 +148,8 @@ PyObject *step_rows(PyObject *, PyObject *args) {
         if (masters && type != at::kFloat) {
           w = entry(st, k_master);
           if (!w || !fits(*w, at::kFloat, device, n)) return other_case();
+        } else if (PyDict_GetItemWithError(st, k_master)) {
+          return other_case();  // master weights that the step would leave behind
         }
         Bucket *b = nullptr;
         for (Bucket &x : buckets)

@@ -212,14 +212,15 @@ class FusedAdamW(torch.optim.Optimizer):
                     per 128 elements (include/fsgs.h, fsgs_adamw_step); 2.02 bytes an element instead of 8.  `moments()`
                     and `set_moments()` convert.  Changing a group's state_bits converts its moments at the next step.
     master_weights  float32 copies of 16-bit parameters in state[p]['master'], which the step updates; the parameter is the
-                    copy rounded to nearest.  Made from the parameter at its first step.
+                    copy rounded to nearest.  Made from the parameter at its first step: after writing to a parameter by
+                    hand, delete its 'master'.
     maximize        ascend.
     capturable      'step' is a 0-d float32 tensor on the parameter's device and lr may be one too, so that a step captured
                     into a graph counts on at every replay.  A step of any other group inside a capture is refused.  Run one
                     eager step before the capture: it makes the state.
     max_grad_norm   bound on the 2-norm over the gradients of ALL groups (one device then): the step uses the gradients times
                     min(1, max_grad_norm / (norm + 1e-6)) and leaves .grad as it is; `last_grad_norm` is that norm, 0-d on
-                    the device."""
+                    the device.  Not part of state_dict()."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, maximize=False, state_bits=32,
                  master_weights=False, capturable=False, max_grad_norm=None):
@@ -241,6 +242,9 @@ class FusedAdamW(torch.optim.Optimizer):
         except Exception:
             self.param_groups.pop()
             raise
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm}
 
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -450,7 +454,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 rc = lib.fsgs_adamw_step(n, rows, len(hypers) // _lib.ADAMW_HYPER_BYTES, hypers, b.dtype, b.bits, b.maximize, coef,
                                          _lib.ptr(scratch), _lib.current_stream())
                 if rc == _lib.FSGS_ERR_INVALID:
-                    raise ValueError("FusedAdamW: two of the tensors of a step share memory")
+                    raise ValueError("FusedAdamW: two of the tensors of a step share memory (or one has over 2^34 elements)")
                 _lib.check(rc, "fsgs_adamw_step")
             _lib.host().stepped(b.params, b.states)
         return loss
@@ -511,6 +515,8 @@ class FusedAdamW(torch.optim.Optimizer):
                     if w.dtype != _F32 or w.device != dev or not _same_layout(w, p):
                         raise ValueError("FusedAdamW: state['master'] is a float32 tensor of the parameter's shape and strides")
                     master = w.data_ptr()
+                else:
+                    st.pop("master", None)  # it would be out of date from this step on
                 key = (dev, dt, bits, use_master, bool(group["maximize"]), capturable)
                 b = buckets.get(key)
                 if b is None:

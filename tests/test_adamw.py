@@ -189,6 +189,18 @@ def test_state_dict_keeps_every_entrys_type():
     assert torch.equal(st["master"], opt.state[p]["master"])
 
 
+def test_copies_and_pickles_keep_the_bound():
+    import copy
+    import pickle
+
+    opt = FusedAdamW([leaf(3)], max_grad_norm=0.5, state_bits=8)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert other.max_grad_norm == 0.5 and other.last_grad_norm is None and other.param_groups[0]["state_bits"] == 8
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            other.param_groups[0]["params"][0].grad = torch.ones(3)
+            other.step()
+
+
 def test_the_cloud_takes_adamw_and_keeps_it():
     from fsgs_amd import synth
     from fsgs_amd.model import GaussianCloud

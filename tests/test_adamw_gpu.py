@@ -585,6 +585,50 @@ def test_changing_the_width_and_saving():
     assert "exp_avg" not in other.state[qs[0]] and other.state[qs[0]]["step"] == 3
 
 
+def test_masters_that_are_switched_off_and_on_start_from_the_parameter():
+    p = torch.ones(50, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    p.grad = torch.ones(50, device=DEV, dtype=torch.bfloat16)
+    opt = FusedAdamW([p], lr=1e-1, master_weights=True, weight_decay=0.0)
+    opt.step()
+    opt.param_groups[0]["master_weights"] = False
+    for _ in range(3):
+        opt.step()
+    assert "master" not in opt.state[p]
+    before = p.detach().float()
+    opt.param_groups[0]["master_weights"] = True
+    opt.step()
+    assert float((opt.state[p]["master"] - (before - 0.1)).abs().max()) < 1e-5  # a constant gradient moves by lr a step
+
+
+def test_saved_states_load_without_unpickling(tmp_path):
+    ps, gs = make([300, 7], torch.float16, seed=8)
+    opt = FusedAdamW(ps, state_bits=8, master_weights=True, eps=1e-6)
+    for p, g in zip(ps, gs):
+        p.grad = g
+    opt.step()
+    torch.save(opt.state_dict(), os.path.join(str(tmp_path), "opt.pth"))
+    qs = [p.detach().clone().requires_grad_(True) for p in ps]
+    other = FusedAdamW(qs, state_bits=8, master_weights=True, eps=1e-6)
+    other.load_state_dict(torch.load(os.path.join(str(tmp_path), "opt.pth"), weights_only=True))
+    for q, g in zip(qs, gs):
+        q.grad = g
+    opt.step(), other.step()
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q) and torch.equal(opt.state[p]["master"], other.state[q]["master"])
+
+
+def test_a_norm_over_more_than_4_g_elements():
+    n = 2 ** 32 + 4099
+    g = torch.zeros(n, device=DEV, dtype=torch.float16)
+    g[-3:], g[2 ** 31], g[0] = 2.0, 1.0, 4.0
+    p = torch.zeros(n, device=DEV, dtype=torch.float16, requires_grad=True)
+    p.grad = g
+    want = math.sqrt(3 * 4 + 1 + 16)
+    assert abs(float(clip_grad_norm_([p], want / 2)) - want) <= 2 * E32 * want
+    for at, v in ((-1, 1.0), (-3, 1.0), (2 ** 31, 0.5), (0, 2.0), (1, 0.0), (-4, 0.0)):
+        assert abs(float(g[at]) - v) < 1e-3
+
+
 def test_offsets_over_32_bits():
     """one bf16 tensor of 2^31 + 4099 elements with 8-bit moments (17 GB in all): its last elements equal those of a small
     tensor whose blocks hold the same values, where the thresholds are the same"""
