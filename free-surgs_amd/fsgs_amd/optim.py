@@ -126,6 +126,7 @@ def _grad_table(params, who):
     return _table_of([p.grad for p in params if p.grad is not None], who)
 
 
+@torch.no_grad()
 def _table_of(grads, who):
     dev, table, keep, dense = _one_device(grads, who), array("q"), [], True
     for g in grads:
@@ -154,7 +155,6 @@ def _max_norm(v):
     return v
 
 
-@torch.no_grad()
 def grad_norm(tensors):
     """Global 2-norm of any number of float32 / bfloat16 / float16 tensors on one device: a 0-d float32 tensor there, no host
     synchronisation.  Squares are summed in 64 bits and in a fixed order."""
@@ -169,7 +169,6 @@ def grad_norm(tensors):
     return norm
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ in three launches per 192 tensors: the gradients' global 2-norm, and every gradient
     (dense, on one device, float32 / bfloat16 / float16 side by side) scaled in place by min(1, max_norm / (norm + 1e-6));
@@ -426,7 +425,6 @@ class FusedAdamW(torch.optim.Optimizer):
                     self.state[p][k] = v.detach().to(p.device, copy=True)
 
     # ---- the step -----------------------------------------------------------------------------------------------------
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -462,14 +460,13 @@ class FusedAdamW(torch.optim.Optimizer):
     def _ordinary(self):
         """The buckets of a step whose tensors and options are all as one expects them -- packed tensors with their states in
         place, options that are plain numbers in range -- collected by the host extension; None where anything is not."""
-        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
-            return None
         found = _lib.host().step_rows(self.param_groups, self.state)
-        if found is None:
+        if found is None or (found and torch.cuda.is_current_stream_capturing()):
             return None
         return [_Bucket(torch.device("cuda", index), dtype, bits, maximize, False, rows, hypers, params, states)
                 for index, dtype, bits, maximize, rows, hypers, params, states in found]
 
+    @torch.no_grad()
     def _general(self):
         """The buckets of any step that can be made: every tensor looked at in turn; states made or converted."""
         capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
