@@ -46,6 +46,7 @@ const at::Tensor *entry(PyObject *state, PyObject *key) {  // state[key] as a pl
 struct Ref {  // an owned reference
   PyObject *o;
   explicit Ref(PyObject *p) : o(p) {}
+  static PyObject *more(PyObject *p) { Py_XINCREF(p); return p; }
   ~Ref() { Py_XDECREF(o); }
   PyObject *release() { PyObject *p = o; o = nullptr; return p; }
   Ref(const Ref &) = delete;
@@ -122,11 +123,14 @@ PyObject *step_rows(PyObject *, PyObject *args) {
         return other_case();
       PyObject *const km = bits == 8 ? k_mq : k_m, *const kv = bits == 8 ? k_vq : k_v;
       const at::ScalarType moment = bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
+      // a parameter's hash is Python code, during which other threads may run: what is used after it is held
+      const Ref hold_list(Ref::more(list));
       for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); i++) {
         PyObject *o = PyList_GET_ITEM(list, i);
         if (!plain(o)) return other_case();
+        const Ref hold(Ref::more(o));
         const at::Tensor &p = THPVariable_Unpack(o);
-        const at::Tensor &g = p.grad();
+        const at::Tensor g = p.grad();
         if (!g.defined()) continue;
         const at::ScalarType type = p.scalar_type();
         const c10::Device device = p.device();
@@ -248,14 +252,17 @@ PyObject *moment_rows(PyObject *, PyObject *args) {
   if (!THPDtype_Check(dtype)) { PyErr_SetString(PyExc_TypeError, "a dtype"); return nullptr; }
   return guarded([&]() -> PyObject * {
     const at::ScalarType type = ((THPDtype *)dtype)->scalar_type;
-    struct Item { const at::Tensor *m, *v, *s; };
+    struct Item { at::Tensor m, v, s; };  // held, as in step_rows
     std::vector<Item> items;
     c10::Device device(c10::kCPU);
     for (Py_ssize_t k = 0; k < PyList_GET_SIZE(groups); k++) {
       PyObject *group = PyList_GET_ITEM(groups, k), *list = PyDict_Check(group) ? PyDict_GetItemWithError(group, k_params) : nullptr;
       if (!list || !PyList_Check(list)) return other_case();
+      const Ref hold_list(Ref::more(list));
       for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); i++) {
-        PyObject *o = PyList_GET_ITEM(list, i), *st = PyDict_GetItemWithError(state, o);
+        PyObject *o = PyList_GET_ITEM(list, i);
+        const Ref hold(Ref::more(o));
+        PyObject *st = PyDict_GetItemWithError(state, o);
         if (PyErr_Occurred()) return nullptr;
         if (!st) continue;
         if (!plain(o) || !PyDict_Check(st)) return other_case();
@@ -267,7 +274,7 @@ PyObject *moment_rows(PyObject *, PyObject *args) {
             mq->sizes() != THPVariable_Unpack(o).sizes() ||
             !fits(*s, at::kByte, device, 2 * ((n + FSGS_ADAMW_BLOCK - 1) / FSGS_ADAMW_BLOCK)))
           return other_case();
-        items.push_back({mq, vq, s});
+        items.push_back({*mq, *vq, *s});
       }
     }
     if (items.empty()) return other_case();
@@ -278,9 +285,9 @@ PyObject *moment_rows(PyObject *, PyObject *args) {
     for (size_t i = 0; i < items.size(); i++) {
       const Item &x = items[i];
       // torch's own function behind torch.empty, without an operator's dispatch for each of what may be hundreds
-      const at::Tensor m(at::detail::empty_cuda(x.m->sizes(), type, device, std::nullopt)),
-          v(at::detail::empty_cuda(x.m->sizes(), type, device, std::nullopt));
-      const int64_t row[] = {address(*x.m), address(*x.v), address(*x.s), address(m), address(v), x.m->numel()};
+      const at::Tensor m(at::detail::empty_cuda(x.m.sizes(), type, device, std::nullopt)),
+          v(at::detail::empty_cuda(x.m.sizes(), type, device, std::nullopt));
+      const int64_t row[] = {address(x.m), address(x.v), address(x.s), address(m), address(v), x.m.numel()};
       static_assert(sizeof(row) == sizeof(FsgsAdamWMoments), "a row");
       rows.insert(rows.end(), row, row + 6);
       Ref a(THPVariable_Wrap(m)), b(THPVariable_Wrap(v));

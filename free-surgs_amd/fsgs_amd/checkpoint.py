@@ -75,7 +75,7 @@ def restore_gaussians(pc, model_args, opt=OptimizationParams, eps=1e-15, fused=T
     pc.variables["xyz_gradient_accum"] = torch.zeros_like(plain(model_args[8]))
     pc.variables["denom"] = torch.zeros_like(plain(model_args[9]))
     pc.spatial_lr_scale = float(model_args[11])
-    pc.training_setup(opt, eps=eps, fused=fused, adamw=pc.adamw)
+    pc.training_setup(opt, eps=eps, fused=fused, adamw=getattr(pc, "adamw", None))
     sd = model_args[10]
     pc.optimizer.load_state_dict({
         "param_groups": sd["param_groups"],

@@ -156,8 +156,8 @@ def _max_norm(v):
 
 
 def grad_norm(tensors):
-    """Global 2-norm of any number of float32 / bfloat16 / float16 tensors on one device: a 0-d float32 tensor there, no host
-    synchronisation.  Squares are summed in 64 bits and in a fixed order."""
+    """Global 2-norm of any number of float32 / bfloat16 / float16 tensors on one device: a 0-d float32 tensor there, without a
+    gradient and without a host synchronisation.  Squares are summed in 64 bits and in a fixed order."""
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
     if not tensors:
         return torch.tensor(0.0)
@@ -218,8 +218,9 @@ class FusedAdamW(torch.optim.Optimizer):
                     into a graph counts on at every replay.  A step of any other group inside a capture is refused.  Run one
                     eager step before the capture: it makes the state.
     max_grad_norm   bound on the 2-norm over the gradients of ALL groups (one device then): the step uses the gradients times
-                    min(1, max_grad_norm / (norm + 1e-6)) and leaves .grad as it is; `last_grad_norm` is that norm, 0-d on
-                    the device.  Not part of state_dict()."""
+                    min(1, max_grad_norm / (norm + 1e-6)) and leaves .grad as it is (a NaN among them makes every parameter
+                    NaN, as clip_grad_norm_ in front of a step does); `last_grad_norm` is that norm, 0-d on the device.
+                    Not part of state_dict()."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, maximize=False, state_bits=32,
                  master_weights=False, capturable=False, max_grad_norm=None):
@@ -422,7 +423,11 @@ class FusedAdamW(torch.optim.Optimizer):
         for i, p in zip(saved, mine):
             for k, v in state_dict["state"].get(i, {}).items():
                 if torch.is_tensor(v) and k != "step":
-                    self.state[p][k] = v.detach().to(p.device, copy=True)
+                    if v.dtype == _F32 and v.shape == p.shape:  # whatever layout it was saved in
+                        self.state[p][k] = torch.empty_like(p, dtype=_F32, memory_format=torch.preserve_format,
+                                                            requires_grad=False).copy_(v.detach())
+                    else:
+                        self.state[p][k] = v.detach().to(p.device, copy=True)
 
     # ---- the step -----------------------------------------------------------------------------------------------------
     def step(self, closure=None):

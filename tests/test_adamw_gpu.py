@@ -600,6 +600,19 @@ def test_masters_that_are_switched_off_and_on_start_from_the_parameter():
     assert float((opt.state[p]["master"] - (before - 0.1)).abs().max()) < 1e-5  # a constant gradient moves by lr a step
 
 
+def test_moments_saved_in_another_layout_load():
+    p = torch.randn(6, 5, device=DEV).requires_grad_(True)
+    opt = FusedAdamW([p])
+    p.grad = torch.randn(6, 5, device=DEV)
+    opt.step()
+    q = p.detach().t().contiguous().t().requires_grad_(True)
+    other = FusedAdamW([q])
+    other.load_state_dict(opt.state_dict())
+    q.grad = p.grad
+    opt.step(), other.step()
+    assert other.state[q]["exp_avg"].stride() == q.stride() and torch.equal(p, q)
+
+
 def test_saved_states_load_without_unpickling(tmp_path):
     ps, gs = make([300, 7], torch.float16, seed=8)
     opt = FusedAdamW(ps, state_bits=8, master_weights=True, eps=1e-6)
@@ -630,8 +643,8 @@ def test_a_norm_over_more_than_4_g_elements():
 
 
 def test_offsets_over_32_bits():
-    """one bf16 tensor of 2^31 + 4099 elements with 8-bit moments (17 GB in all): its last elements equal those of a small
-    tensor whose blocks hold the same values, where the thresholds are the same"""
+    """one bf16 tensor of 2^31 + 4099 elements with 8-bit moments (13 GB in all), then with 32-bit ones (26 GB): gradients in its
+    last elements alone"""
     n, tail = 2 ** 31 + 4099, 4099
     p = torch.zeros(n, device=DEV, dtype=torch.bfloat16, requires_grad=True)
     p.grad = torch.zeros(n, device=DEV, dtype=torch.bfloat16)
@@ -648,6 +661,12 @@ def test_offsets_over_32_bits():
     u = thresholds(tail, 1, GOLDEN, 0, n - tail)
     check_codes(st["exp_avg_q"].view(torch.uint8)[n - tail:], st["scales"][(n - tail) // 128:, 0], m1, 12 * E32 * m1.abs(), u, False, "m")
     assert bool((p.detach()[:100000] == 0).all()) and not bool(st["exp_avg_q"].view(torch.uint8)[:n - tail].any())
+    del opt, st
+    opt32 = FusedAdamW([p], state_bits=32, max_grad_norm=1.0, lr=1e-2)
+    p.detach().zero_()
+    opt32.step()
+    close(opt32.state[p]["exp_avg"][n - tail:], m1, 12 * E32 * m1.abs(), "m")
+    assert not bool(opt32.state[p]["exp_avg_sq"][:n - tail].any())
     step = torch.where(g == 0, torch.zeros_like(g), -1e-2 * g.sign())
     assert float((p.detach()[n - tail:] - step).abs().max()) < 1e-4  # the first step is lr whatever the gradient's size
 
