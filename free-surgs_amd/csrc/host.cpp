@@ -206,8 +206,12 @@ PyObject *stepped(PyObject *, PyObject *args) {
   });
 }
 
-// grad_rows(params) -> (rows, device index) of the gradients that there are, or None; all on one device
-PyObject *grad_rows(PyObject *, PyObject *params) {
+// grad_rows(params, nbytes) -> (rows, device index, norm, scratch) of the gradients that there are, or None; all on one device.
+// norm, scratch: a new 0-d float32 tensor and one of nbytes bytes there, None without gradients.
+PyObject *grad_rows(PyObject *, PyObject *args) {
+  PyObject *params;
+  long long nbytes;
+  if (!PyArg_ParseTuple(args, "OL", &params, &nbytes)) return nullptr;
   if (!PyList_Check(params)) Py_RETURN_NONE;
   return guarded([&]() -> PyObject * {
     std::vector<int64_t> rows;
@@ -226,7 +230,12 @@ PyObject *grad_rows(PyObject *, PyObject *params) {
     }
     Ref bytes(rows_of(rows));
     if (!bytes.o) return nullptr;
-    return Py_BuildValue("(Oi)", bytes.o, device);
+    if (device < 0) return Py_BuildValue("(OiOO)", bytes.o, device, Py_None, Py_None);
+    const c10::Device on(c10::kCUDA, (c10::DeviceIndex)device);
+    Ref norm(THPVariable_Wrap(at::Tensor(at::detail::empty_cuda({}, at::kFloat, on, std::nullopt)))),
+        scratch(THPVariable_Wrap(at::Tensor(at::detail::empty_cuda({(int64_t)nbytes}, at::kByte, on, std::nullopt))));
+    if (!norm.o || !scratch.o) return nullptr;
+    return Py_BuildValue("(OiOO)", bytes.o, device, norm.o, scratch.o);
   });
 }
 
@@ -305,7 +314,7 @@ PyObject *moment_rows(PyObject *, PyObject *args) {
 PyMethodDef methods[] = {
     {"step_rows", step_rows, METH_VARARGS, "the launch sequences of an ordinary step, or None"},
     {"stepped", stepped, METH_VARARGS, "count a step in every state and raise the parameters' versions"},
-    {"grad_rows", grad_rows, METH_O, "(rows, device) of the parameters' gradients, or None"},
+    {"grad_rows", grad_rows, METH_VARARGS, "(rows, device, norm, scratch) for the parameters' gradients, or None"},
     {"grads_written", grads_written, METH_O, "raise the versions of the parameters' gradients"},
     {"moment_rows", moment_rows, METH_VARARGS, "(pairs, rows, device) of the 8-bit moments of all parameters, or None"},
     {nullptr, nullptr, 0, nullptr}};

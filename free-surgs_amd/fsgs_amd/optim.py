@@ -106,28 +106,38 @@ def _check_grad(g, name="gradient"):
         raise TypeError("%s: float32, bfloat16 or float16, got %s" % (name, g.dtype))
 
 
-def _norm_of(entry, dev, table, max_norm):
-    """(return code, norm, tensor whose first float is the factor) of fsgs_grad_norm / _clip on the gradients in a table
-    (rows of FsgsGradTensor, as bytes), on dev's current stream"""
-    n = len(table) // (8 * _lib.GRAD_TENSOR_WORDS)
-    nbytes = _lib.load().fsgs_grad_norm_scratch_bytes(n)
-    norm = torch.empty((), dtype=_F32, device=dev)
-    scratch = torch.empty(16 + nbytes, dtype=torch.uint8, device=dev)
-    factor = scratch.data_ptr()
-    return entry(n, table, max_norm, factor + 16, nbytes, norm.data_ptr(), factor, _lib.current_stream()), norm, scratch
+class _Grads:
+    """what a norm's launches need: rows of FsgsGradTensor as bytes, on one device (None: no gradients), the tensor for the norm,
+    scratch whose first float is the factor; `dense`: whether all are; `slow`: what to keep until the launch, None where all
+    were as one expects"""
+
+    def __init__(self, device, table, norm, scratch, dense=True, slow=None):
+        self.device, self.table, self.norm, self.scratch, self.dense, self.slow = device, table, norm, scratch, dense, slow
+
+    def __len__(self):
+        return len(self.table) // (8 * _lib.GRAD_TENSOR_WORDS)
+
+    def launch(self, entry, max_norm):
+        """the return code of fsgs_grad_norm / _clip, on the device's current stream (the device has been made current)"""
+        at = self.factor = self.scratch.data_ptr()
+        return entry(len(self), self.table, max_norm, at + 16, self.scratch.numel() - 16, self.norm.data_ptr(), at,
+                     _lib.current_stream())
 
 
-def _grad_table(params, who):
-    """(device, rows, whether all are packed, what to keep until the launch) of the gradients of params; the device is None
-    where there are none"""
-    fast = _lib.host().grad_rows(params)
+def _scratch_bytes(n):
+    return 16 + _lib.load().fsgs_grad_norm_scratch_bytes(n)
+
+
+def _grads_of(params, who):
+    fast = _lib.host().grad_rows(params, _scratch_bytes(len(params)))
     if fast is not None:
-        return (torch.device("cuda", fast[1]) if fast[1] >= 0 else None), fast[0], True, None
-    return _table_of([p.grad for p in params if p.grad is not None], who)
+        table, index, norm, scratch = fast
+        return _Grads(torch.device("cuda", index) if index >= 0 else None, table, norm, scratch)
+    return _grads_from([p.grad for p in params if p.grad is not None], who)
 
 
 @torch.no_grad()
-def _table_of(grads, who):
+def _grads_from(grads, who):
     dev, table, keep, dense = _one_device(grads, who), array("q"), [], True
     for g in grads:
         if g.is_neg():
@@ -136,7 +146,8 @@ def _table_of(grads, who):
             dense, g = False, g.contiguous()
             keep.append(g)
         table.extend((g.data_ptr(), g.numel(), _DTYPES[g.dtype]))
-    return dev, table.tobytes(), dense, keep
+    return _Grads(dev, table.tobytes(), torch.empty((), dtype=_F32, device=dev),
+                  torch.empty(_scratch_bytes(len(grads)), dtype=torch.uint8, device=dev), dense, keep)
 
 
 def _one_device(grads, who):
@@ -161,12 +172,10 @@ def grad_norm(tensors):
     tensors = [tensors] if torch.is_tensor(tensors) else list(tensors)
     if not tensors:
         return torch.tensor(0.0)
-    lib = _lib.load()
-    dev, table, _, _keep = _table_of(tensors, "grad_norm")
-    with _on(dev):
-        rc, norm, _ = _norm_of(lib.fsgs_grad_norm, dev, table, float("inf"))
-    _lib.check(rc, "fsgs_grad_norm")
-    return norm
+    found = _grads_from(tensors, "grad_norm")
+    with _on(found.device):
+        _lib.check(found.launch(_lib.load().fsgs_grad_norm, float("inf")), "fsgs_grad_norm")
+    return found.norm
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -179,25 +188,25 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     max_norm = _max_norm(max_norm)
     parameters = [parameters] if torch.is_tensor(parameters) else list(parameters)
     lib = _lib.load()
-    dev, table, dense, slow = _grad_table(parameters, "clip_grad_norm_")
-    if dev is None:
+    found = _grads_of(parameters, "clip_grad_norm_")
+    if found.device is None:
         return torch.tensor(0.0)
-    if not dense:
+    if not found.dense:
         raise ValueError("clip_grad_norm_: gradients are dense in memory; scale slices of other tensors by hand")
-    with _on(dev):
-        rc, norm, factor = _norm_of(lib.fsgs_grad_norm if error_if_nonfinite else lib.fsgs_grad_clip, dev, table, max_norm)
+    with _on(found.device):
+        rc = found.launch(lib.fsgs_grad_norm if error_if_nonfinite else lib.fsgs_grad_clip, max_norm)
         if error_if_nonfinite and rc == _lib.FSGS_OK:
-            if not bool(torch.isfinite(norm)):
-                raise RuntimeError("clip_grad_norm_: the gradients' norm is %s" % float(norm))
-            rc = lib.fsgs_grad_scale(len(table) // (8 * _lib.GRAD_TENSOR_WORDS), table, factor.data_ptr(), _lib.current_stream())
+            if not bool(torch.isfinite(found.norm)):
+                raise RuntimeError("clip_grad_norm_: the gradients' norm is %s" % float(found.norm))
+            rc = lib.fsgs_grad_scale(len(found), found.table, found.factor, _lib.current_stream())
         if rc == _lib.FSGS_ERR_INVALID:
             raise ValueError("clip_grad_norm_: two of the gradients share memory, or a parameter is given twice")
         _lib.check(rc, "fsgs_grad_clip")
-    if slow is None:
+    if found.slow is None:
         _lib.host().grads_written(parameters)
     else:
         mark_updated([p.grad for p in parameters if p.grad is not None])
-    return norm
+    return found.norm
 
 
 class FusedAdamW(torch.optim.Optimizer):
@@ -444,11 +453,10 @@ class FusedAdamW(torch.optim.Optimizer):
         coef = None
         if self.max_grad_norm is not None:
             params = work[0].params if len(work) == 1 else [p for bucket in work for p in bucket.params]
-            dev, table, _, _keep = _grad_table(params, "FusedAdamW(max_grad_norm)")
-            with _on(dev):
-                rc, self.last_grad_norm, factor = _norm_of(lib.fsgs_grad_norm, dev, table, self.max_grad_norm)
-            _lib.check(rc, "fsgs_grad_norm")
-            coef = factor.data_ptr()
+            found = _grads_of(params, "FusedAdamW(max_grad_norm)")
+            with _on(found.device):
+                _lib.check(found.launch(lib.fsgs_grad_norm, self.max_grad_norm), "fsgs_grad_norm")
+            self.last_grad_norm, coef = found.norm, found.factor
         for b in work:
             n = len(b.params)
             rows, hypers = b.arrays()
