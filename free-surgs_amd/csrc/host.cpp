@@ -53,6 +53,12 @@ struct Ref {  // an owned reference
   Ref &operator=(const Ref &) = delete;
 };
 
+// torch's own function behind torch.empty, without the dispatch of an operator
+PyObject *fresh(at::IntArrayRef sizes, at::ScalarType type, int device) {
+  return THPVariable_Wrap(at::Tensor(
+      at::detail::empty_cuda(sizes, type, c10::Device(c10::kCUDA, (c10::DeviceIndex)device), std::nullopt)));
+}
+
 PyObject *rows_of(const std::vector<int64_t> &rows) {
   return PyBytes_FromStringAndSize((const char *)rows.data(), (Py_ssize_t)(rows.size() * sizeof(int64_t)));
 }
@@ -231,11 +237,20 @@ PyObject *grad_rows(PyObject *, PyObject *args) {
     Ref bytes(rows_of(rows));
     if (!bytes.o) return nullptr;
     if (device < 0) return Py_BuildValue("(OiOO)", bytes.o, device, Py_None, Py_None);
-    const c10::Device on(c10::kCUDA, (c10::DeviceIndex)device);
-    Ref norm(THPVariable_Wrap(at::Tensor(at::detail::empty_cuda({}, at::kFloat, on, std::nullopt)))),
-        scratch(THPVariable_Wrap(at::Tensor(at::detail::empty_cuda({(int64_t)nbytes}, at::kByte, on, std::nullopt))));
+    Ref norm(fresh({}, at::kFloat, device)), scratch(fresh({(int64_t)nbytes}, at::kByte, device));
     if (!norm.o || !scratch.o) return nullptr;
     return Py_BuildValue("(OiOO)", bytes.o, device, norm.o, scratch.o);
+  });
+}
+
+// norm_buffers(device index, nbytes) -> (norm, scratch): a new 0-d float32 tensor and one of nbytes bytes
+PyObject *norm_buffers(PyObject *, PyObject *args) {
+  int device;
+  long long nbytes;
+  if (!PyArg_ParseTuple(args, "iL", &device, &nbytes)) return nullptr;
+  return guarded([&]() -> PyObject * {
+    Ref norm(fresh({}, at::kFloat, device)), scratch(fresh({(int64_t)nbytes}, at::kByte, device));
+    return norm.o && scratch.o ? PyTuple_Pack(2, norm.o, scratch.o) : nullptr;
   });
 }
 
@@ -293,14 +308,12 @@ PyObject *moment_rows(PyObject *, PyObject *args) {
     rows.reserve(6 * items.size());
     for (size_t i = 0; i < items.size(); i++) {
       const Item &x = items[i];
-      // torch's own function behind torch.empty, without an operator's dispatch for each of what may be hundreds
-      const at::Tensor m(at::detail::empty_cuda(x.m.sizes(), type, device, std::nullopt)),
-          v(at::detail::empty_cuda(x.m.sizes(), type, device, std::nullopt));
-      const int64_t row[] = {address(x.m), address(x.v), address(x.s), address(m), address(v), x.m.numel()};
+      Ref a(fresh(x.m.sizes(), type, device.index())), b(fresh(x.m.sizes(), type, device.index()));
+      if (!a.o || !b.o) return nullptr;
+      const int64_t row[] = {address(x.m), address(x.v), address(x.s), address(THPVariable_Unpack(a.o)),
+                             address(THPVariable_Unpack(b.o)), x.m.numel()};
       static_assert(sizeof(row) == sizeof(FsgsAdamWMoments), "a row");
       rows.insert(rows.end(), row, row + 6);
-      Ref a(THPVariable_Wrap(m)), b(THPVariable_Wrap(v));
-      if (!a.o || !b.o) return nullptr;
       PyObject *pair = PyTuple_Pack(2, a.o, b.o);
       if (!pair) return nullptr;
       PyList_SET_ITEM(pairs.o, (Py_ssize_t)i, pair);
@@ -315,6 +328,7 @@ PyMethodDef methods[] = {
     {"step_rows", step_rows, METH_VARARGS, "the launch sequences of an ordinary step, or None"},
     {"stepped", stepped, METH_VARARGS, "count a step in every state and raise the parameters' versions"},
     {"grad_rows", grad_rows, METH_VARARGS, "(rows, device, norm, scratch) for the parameters' gradients, or None"},
+    {"norm_buffers", norm_buffers, METH_VARARGS, "(norm, scratch) on a device"},
     {"grads_written", grads_written, METH_O, "raise the versions of the parameters' gradients"},
     {"moment_rows", moment_rows, METH_VARARGS, "(pairs, rows, device) of the 8-bit moments of all parameters, or None"},
     {nullptr, nullptr, 0, nullptr}};

@@ -198,7 +198,7 @@ _PROTOTYPES = {
     "fsgs_pose_frame_begin": (_i, [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "fsgs_adam_step": (_i, [_i, C.POINTER(FsgsAdamGroup), C.c_double, C.c_double, C.c_double, _vp]),
     "fsgs_adamw_scratch_bytes": (_sz, [_i]),
-    "fsgs_adamw_step": (_i, [_i, _vp, _i, _vp, _i, _i, _i, _vp, _vp, _vp]),
+    "fsgs_adamw_step": (_i, [_i, _vp, _i, _vp, _i, _i, _i, _vp, C.c_float, _vp, _vp, _sz, _vp, _vp]),
     "fsgs_adamw_moments": (_i, [_i, _vp, _i, _i, _vp]),
     "fsgs_grad_norm_scratch_bytes": (_sz, [_i]),
     "fsgs_grad_norm": (_i, [_i, _vp, C.c_float, _vp, _sz, _vp, _vp, _vp]),

@@ -450,19 +450,24 @@ class FusedAdamW(torch.optim.Optimizer):
             work = self._general()
         if not work:
             return loss
-        coef = None
-        if self.max_grad_norm is not None:
-            params = work[0].params if len(work) == 1 else [p for bucket in work for p in bucket.params]
-            found = _grads_of(params, "FusedAdamW(max_grad_norm)")
+        # (factor, bound, norm, scratch, its bytes): nothing, the bound that a single bucket applies by itself, or the factor
+        # from the norm over several
+        limit = (None, 0.0, None, None, 0)
+        if self.max_grad_norm is not None and len(work) == 1:
+            nbytes = _scratch_bytes(len(work[0].params))
+            norm, hold = _lib.host().norm_buffers(work[0].device.index, nbytes)
+            limit, self.last_grad_norm = (None, self.max_grad_norm, norm.data_ptr(), hold.data_ptr(), nbytes), norm
+        elif self.max_grad_norm is not None:
+            found = hold = _grads_of([p for b in work for p in b.params], "FusedAdamW(max_grad_norm)")
             with _on(found.device):
                 _lib.check(found.launch(lib.fsgs_grad_norm, self.max_grad_norm), "fsgs_grad_norm")
-            self.last_grad_norm, coef = found.norm, found.factor
+            limit, self.last_grad_norm = (found.factor, 0.0, None, None, 0), found.norm
         for b in work:
             n = len(b.params)
             rows, hypers = b.arrays()
             with _on(b.device):
                 scratch = torch.empty(lib.fsgs_adamw_scratch_bytes(n), dtype=torch.uint8, device=b.device) if b.capturable else None
-                rc = lib.fsgs_adamw_step(n, rows, len(hypers) // _lib.ADAMW_HYPER_BYTES, hypers, b.dtype, b.bits, b.maximize, coef,
+                rc = lib.fsgs_adamw_step(n, rows, len(hypers) // _lib.ADAMW_HYPER_BYTES, hypers, b.dtype, b.bits, b.maximize, *limit,
                                          _lib.ptr(scratch), _lib.current_stream())
                 if rc == _lib.FSGS_ERR_INVALID:
                     raise ValueError("FusedAdamW: two of the tensors of a step share memory (or one has over 2^34 elements)")

@@ -544,10 +544,13 @@ typedef struct FsgsAdamWHyper {
 } FsgsAdamWHyper;
 /* bytes of the scratch that a call with step_dev needs (kept until its kernels have run) */
 size_t fsgs_adamw_scratch_bytes(int n_tensors);
-/* tensors, hypers: HOST arrays.  grad_coef: float[1] DEVICE factor on the gradients (`factor` of fsgs_grad_norm) or NULL.
+/* tensors, hypers: HOST arrays.  The factor on the gradients is one of: grad_factor, float[1] on the DEVICE (`factor` of
+ * fsgs_grad_norm); with norm (float[1] on the DEVICE, else NULL) min(1, max_norm / (norm + 1e-6)) for the 2-norm over this
+ * call's gradients, which is left in *norm; 1.  norm_scratch: 16 + fsgs_grad_norm_scratch_bytes(n_tensors), with norm.
  * scratch: NULL without step_dev. */
 int fsgs_adamw_step(int n_tensors, const FsgsAdamWTensor *tensors, int n_hypers, const FsgsAdamWHyper *hypers, int dtype,
-                    int state_bits, int maximize, const float *grad_coef, void *scratch, fsgs_stream_t stream);
+                    int state_bits, int maximize, const float *grad_factor, float max_norm, float *norm, void *norm_scratch,
+                    size_t norm_scratch_bytes, void *scratch, fsgs_stream_t stream);
 /* 8-bit moments to values (write = 0; exp_avg / exp_avg_sq of `dtype`; bf16 and fp32 hold them exactly) or values (fp32) to
  * codes, rounded to nearest (write = 1). */
 typedef struct FsgsAdamWMoments {
@@ -575,7 +578,7 @@ int fsgs_grad_norm(int n_tensors, const FsgsGradTensor *grads, float max_norm, v
 /* grad *= factor[0] (DEVICE) in place, rounded to the gradient's type; a factor of exactly 1 moves no data.  No two may
  * share memory. */
 int fsgs_grad_scale(int n_tensors, const FsgsGradTensor *grads, const float *factor, fsgs_stream_t stream);
-/* both */
+/* both; `factor` is written only where the call forms it in a launch of its own */
 int fsgs_grad_clip(int n_tensors, const FsgsGradTensor *grads, float max_norm, void *scratch, size_t scratch_bytes,
                    float *norm, float *factor, fsgs_stream_t stream);
 

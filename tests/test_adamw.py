@@ -17,11 +17,11 @@ def hyper(step=1, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, wd=0.0, step_dev=None):
     return _lib.FsgsAdamWHyper(lr, b1, b2, eps, wd, step, step_dev, None)
 
 
-def step(rows, hypers=None, dtype=0, bits=32, scratch=None):
+def step(rows, hypers=None, dtype=0, bits=32, scratch=None, limit=(None, 0.0, None, None, 0)):
     hypers = [hyper()] if hypers is None else hypers
     table = array("q", [w for r in rows for w in r])
     return _lib.load().fsgs_adamw_step(len(rows), table.buffer_info()[0] if rows else None, len(hypers),
-                                       (_lib.FsgsAdamWHyper * len(hypers))(*hypers), dtype, bits, 0, None, scratch, None)
+                                       (_lib.FsgsAdamWHyper * len(hypers))(*hypers), dtype, bits, 0, *limit, scratch, None)
 
 
 def row(k=0, n=100, p=0, g=1, m=2, v=3, scales=4, master=None, h=0):
@@ -51,6 +51,9 @@ def test_step_without_tensors_or_elements_is_a_no_op():
     dict(rows=[(0,) + row()[1:]]), dict(rows=[row()[:1] + (0,) + row()[2:]]),
     dict(rows=[row()[:4] + (0,) + row()[5:]], bits=8),                # no scales
     dict(rows=[row(n=1 << 46)]),                                      # more workgroups than a launch has
+    dict(rows=[row()], limit=(A, 1.0, A + 64, A + 128, 1 << 20)),     # a factor and a bound
+    dict(rows=[row()], limit=(None, -1.0, A + 64, A + 128, 1 << 20)), dict(rows=[row()], limit=(None, float("nan"), A + 64, A + 128, 1 << 20)),
+    dict(rows=[row()], limit=(None, 1.0, A + 64, None, 1 << 20)), dict(rows=[row()], limit=(None, 1.0, A + 64, A + 128, 8)),
     dict(rows=[row()], hypers=[hyper(step_dev=A)]),                   # a step on the device without scratch
     dict(rows=[row(), row(1, h=1)], hypers=[hyper(step_dev=A), hyper()], scratch=A + 64),
     dict(rows=[row(), row(1)], hypers=[hyper(step_dev=A + 8)], scratch=A + 64),  # two tensors on one count
