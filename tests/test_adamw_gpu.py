@@ -562,6 +562,61 @@ def test_streams_and_steps_behind_each_other():
     assert torch.equal(a.state[ps[0]]["exp_avg_q"].view(torch.uint8), b.state[qs[0]]["exp_avg_q"].view(torch.uint8))
 
 
+def test_two_threads_step_at_once():
+    """two optimizers in two threads, each on a stream of its own, against the same steps one after the other"""
+    import threading
+
+    def job(seed, out, stream):
+        ps, gs = make([4097, 50, 300000], torch.bfloat16, seed=seed)
+        opt = FusedAdamW(ps, state_bits=8, master_weights=True, max_grad_norm=0.1)
+        if stream is not None:
+            stream.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(stream):
+            for k in range(40):
+                for p, g in zip(ps, gs):
+                    p.grad = g * (k + 1)
+                opt.step()
+                clip_grad_norm_(ps, 0.5)
+            torch.cuda.current_stream().synchronize()
+        out[seed] = [p.detach() for p in ps] + [t for pair in opt.moments() for t in pair] + [p.grad for p in ps]
+
+    alone, together = {}, {}
+    for seed in (1, 2):
+        job(seed, alone, None)
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=job, args=(seed, together, torch.cuda.Stream())) for seed in (1, 2)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    torch.cuda.synchronize()
+    for seed in (1, 2):
+        assert all(torch.equal(a, b) for a, b in zip(alone[seed], together[seed]))
+
+
+def test_steps_hold_on_to_nothing():
+    import gc
+    import sys
+
+    ps, gs = make([100, 3000], torch.float32, seed=90)
+    opt = FusedAdamW(ps, state_bits=8, max_grad_norm=1.0)
+    for p, g in zip(ps, gs):
+        p.grad = g.clone()
+
+    def once():
+        opt.step(), opt.moments(torch.bfloat16), clip_grad_norm_(ps, 0.5), grad_norm([p.grad for p in ps])
+
+    def held():
+        gc.collect()
+        torch.cuda.synchronize()
+        return ([sys.getrefcount(x) for x in ps + [opt.state, opt.param_groups] + [st for st in opt.state.values()]],
+                [sys.getrefcount(v) for st in opt.state.values() for v in st.values() if torch.is_tensor(v)],
+                torch.cuda.memory_allocated())
+
+    once()
+    before = held()
+    for _ in range(50):
+        once()
+    assert held() == before
+
+
 def test_changing_the_width_and_saving():
     ps, gs = make([1000, 130], torch.bfloat16, seed=50)
     opt = FusedAdamW(ps, state_bits=8, master_weights=True)
