@@ -268,8 +268,10 @@ PyObject *grads_written(PyObject *, PyObject *params) {
   });
 }
 
+int64_t padded(int64_t n) { return (n + 255) / 256 * 256; }
+
 // moment_rows(param_groups, state, dtype) -> ([(m, v)], rows, device index) of the parameters that have a state, in order, or None:
-// new tensors of `dtype` for the values of 8-bit moments
+// tensors of `dtype` for the values of 8-bit moments, cut from one new buffer
 PyObject *moment_rows(PyObject *, PyObject *args) {
   PyObject *groups, *state, *dtype;
   if (!PyArg_ParseTuple(args, "O!O!O", &PyList_Type, &groups, &PyDict_Type, &state, &dtype)) return nullptr;
@@ -306,9 +308,21 @@ PyObject *moment_rows(PyObject *, PyObject *args) {
     if (!pairs.o) return nullptr;
     std::vector<int64_t> rows;
     rows.reserve(6 * items.size());
+    // all values in one allocation, cut on 512-byte boundaries: 0.3 us a tensor where one of its own takes 0.7
+    int64_t total = 0;
+    for (const Item &x : items) total += 2 * padded(x.m.numel());
+    const at::Tensor all(at::detail::empty_cuda({total}, type, device, std::nullopt));
+    int64_t used = 0;
+    const auto cut = [&](at::IntArrayRef sizes, int64_t n) {
+      at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+      t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+      t.unsafeGetTensorImpl()->set_storage_offset(used);
+      used += padded(n);
+      return THPVariable_Wrap(std::move(t));
+    };
     for (size_t i = 0; i < items.size(); i++) {
       const Item &x = items[i];
-      Ref a(fresh(x.m.sizes(), type, device.index())), b(fresh(x.m.sizes(), type, device.index()));
+      Ref a(cut(x.m.sizes(), x.m.numel())), b(cut(x.m.sizes(), x.m.numel()));
       if (!a.o || !b.o) return nullptr;
       const int64_t row[] = {address(x.m), address(x.v), address(x.s), address(THPVariable_Unpack(a.o)),
                              address(THPVariable_Unpack(b.o)), x.m.numel()};

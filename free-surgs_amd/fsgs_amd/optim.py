@@ -367,8 +367,9 @@ class FusedAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def moments(self, dtype=torch.float32):
-        """[(m, v)] of every parameter that has a state, in the order of the groups: new tensors of the parameter's shape in
-        `dtype`.  float32 and bfloat16 hold what 8-bit moments stand for exactly."""
+        """[(m, v)] of every parameter that has a state, in the order of the groups: copies of the parameter's shape in `dtype`.
+        float32 and bfloat16 hold what 8-bit moments stand for exactly.  Those of packed 8-bit states are cut from one new
+        buffer, which lives (and is saved by torch.save) as long as any of them: clone what is to be kept alone."""
         if dtype not in _DTYPES:
             raise TypeError("moments: float32, bfloat16 or float16, got %s" % dtype)
         fast = _lib.host().moment_rows(self.param_groups, self.state, dtype)

@@ -201,6 +201,15 @@ def test_moments_come_back_exactly_and_go_in_to_the_nearest():
         opt.set_moments(p, m, v, 7)
     for (m, v), (m2, v2) in zip(opt.moments(), opt.moments()):
         assert torch.equal(m, m2) and torch.equal(v, v2)
+    pairs = opt.moments()  # cut from one buffer: apart from each other, and whole tensors in every other way
+    spans = sorted((t.data_ptr(), t.data_ptr() + 4 * t.numel()) for pair in pairs for t in pair)
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:])) and all(t.is_contiguous() for pair in pairs for t in pair)
+    keep = pairs[5][1].clone()
+    pairs[5][0].fill_(7.0), pairs[4][1].add_(1.0)
+    assert torch.equal(pairs[5][1], keep) and torch.equal(pairs[5][0].cpu(), torch.full((sizes[5],), 7.0))
+    last = opt.moments()[5][1]
+    del pairs
+    assert torch.equal(last, keep) and last.requires_grad is False and torch.equal(copy.deepcopy(last), keep)
     m16, v16 = opt.moments(torch.float16)[3]
     assert m16.dtype == v16.dtype == torch.float16
 
