@@ -46,10 +46,12 @@ constexpr int THREADS = 256;
 // Elements of one workgroup of a step: two vectors a thread and array.  Four make fewer, larger workgroups (20 k Gaussians,
 // 1.2 M floats: 10.1 us against 8.1; 24 bf16 layers of 20 M in 8 bits: 59 us against 54; no difference at 59 M).
 constexpr int CHUNK = 2048;
-// Bytes of one workgroup's turn: four 16-byte vectors a thread in the norm, two in the scaling (160 bf16 layers of 64 M: norm
-// 27.6 us, with two 30.9, with eight 28.5; scaling 48.0 us, with four 51.7, with one 60.1).
-constexpr int NORM_BYTES = 16384, SCALE_BYTES = 8192;
+// Bytes of one workgroup's turn in the norm, four 16-byte vectors a thread; the scaling's workgroups take half of one (160 bf16
+// layers of 64 M: norm 27.6 us, with two vectors 30.9, with eight 28.5; scaling 48.0 us, with four 51.7, with one 60.1).
+constexpr int NORM_BYTES = 16384, SCALE_BYTES = NORM_BYTES / 2;
+constexpr int XCDS = 8;  // workgroup b of a launch runs on XCD b % 8, which has an L2 of its own
 constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;  // workgroups of one launch (256 threads each: under 2^32 work items)
+constexpr int64_t MAX_TURNS = MAX_BLOCKS / 2 - 8;        // two workgroups of the scaling each, and what fills the last row
 constexpr int QBLOCK = FSGS_ADAMW_BLOCK;  // elements that share a power of two
 constexpr int NORM_GROUPS = 2048;      // workgroups of one norm launch at most: eight per CU
 constexpr int SUMMED = THREADS;        // partial sums that a step or a scaling adds up by itself
@@ -550,9 +552,13 @@ template <typename T, int BYTES, bool WRITE, typename F> __device__ __forceinlin
     }
   }
 }
+__host__ __device__ inline uint32_t scale_rows(uint32_t turns) { return (turns + XCDS - 1) / XCDS; }
+
+// BYTES from `skip` on of turn `at`
 template <int BYTES, bool WRITE, typename F>
-__device__ __forceinline__ void turn_of(const GradTable &t, int k, uint32_t at, F f) {
-  const int64_t nd = t.at[k].n_dtype, n = nd >> 2, done = (int64_t)(at - t.start[k]) * BYTES;
+__device__ __forceinline__ void turn_of(const GradTable &t, uint32_t at, int skip, F f) {
+  const int k = owner<GRADS>(t.start, t.count, at);
+  const int64_t nd = t.at[k].n_dtype, n = nd >> 2, done = (int64_t)(at - t.start[k]) * NORM_BYTES + skip;
   char *g = (char *)t.at[k].g + done;
   if ((nd & 3) == FSGS_DTYPE_F32) turn<float, BYTES, WRITE>((float *)g, 4 * n - done, f);
   else if ((nd & 3) == FSGS_DTYPE_BF16) turn<__bf16, BYTES, WRITE>((__bf16 *)g, 2 * n - done, f);
@@ -580,7 +586,7 @@ __global__ __launch_bounds__(THREADS, 8) void norm_partial_kernel(GradTable t, d
   __shared__ double lds[THREADS / 64];
   Squares sum;
   for (uint32_t at = blockIdx.x; at < t.turns; at += gridDim.x)
-    turn_of<NORM_BYTES, false>(t, owner<GRADS>(t.start, t.count, at), at, [&](const auto &x) { sum(x); });
+    turn_of<NORM_BYTES, false>(t, at, 0, [&](const auto &x) { sum(x); });
   const double s = group_sum<THREADS / 64>(sum.a + sum.b, lds);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
@@ -596,12 +602,17 @@ __global__ __launch_bounds__(1024) void norm_finish_kernel(const double *partial
   }
 }
 
-// 17.7 M floats 22 us = 6.4 TB/s (the norm has just brought part of them into the cache), 64 M bf16 48 us.
-// a factor of exactly 1 leaves every gradient as it is: nothing is read or written then
+// The turns that the norm read last come first, each on the XCD that read it, whose L2 may still hold it: clipping 5.9 M floats
+// 20.0 -> 16.5 us, 17.7 M 37.3 -> 35.6 (the scaling 21 us, 6.7 TB/s), 20 M bf16 25.2 -> 23.4, 64 M bf16 73 -> 71, 59 M floats
+// as before; in the reverse order on any XCD, or on the same XCD in the norm's order, only the smallest gains.
+// A factor of exactly 1 leaves every gradient as it is: nothing is read or written then.
 __global__ __launch_bounds__(THREADS) void grad_scale_kernel(GradTable t, Bound bound) {
   const float c = factor_of(bound);
   if (c == 1.0f) return;
-  turn_of<SCALE_BYTES, true>(t, owner<GRADS>(t.start, t.count, blockIdx.x), blockIdx.x, [&](auto &x) {
+  const uint32_t row = scale_rows(t.turns) - 1 - blockIdx.x / (2 * XCDS), half = blockIdx.x / XCDS % 2;
+  const uint32_t at = row * XCDS + blockIdx.x % XCDS;
+  if (at >= t.turns) return;
+  turn_of<SCALE_BYTES, true>(t, at, half * SCALE_BYTES, [&](auto &x) {
 #pragma unroll
     for (int j = 0; j < (int)(sizeof(x) / sizeof(x[0])); j++) x[j] = (decltype(x[j] + x[j]))((float)x[j] * c);
   });
@@ -636,21 +647,21 @@ struct Regions {
 int64_t chunks_of(int64_t n) { return (n + CHUNK - 1) / CHUNK; }
 int64_t qblocks_of(int64_t n) { return (n + QBLOCK - 1) / QBLOCK; }
 
-int64_t turns_of(const FsgsGradTensor &g, int bytes) { return (g.n * size_of(g.dtype) + bytes - 1) / bytes; }
+int64_t turns_of(const FsgsGradTensor &g) { return (g.n * size_of(g.dtype) + NORM_BYTES - 1) / NORM_BYTES; }
 
-// the next up to 192 gradients (of(i)) from `from` on that make at most MAX_BLOCKS turns; returns the first that is left
-template <typename Of> int fill_grads(GradTable &t, int from, int n_tensors, Of of, int bytes) {
+// the next up to 192 gradients (of(i)) from `from` on that make at most MAX_TURNS turns; returns the first that is left
+template <typename Of> int fill_grads(GradTable &t, int from, int n_tensors, Of of) {
   std::memset(&t, 0, sizeof(t));
   int64_t turns = 0;
   int i = from;
   for (; i < n_tensors && t.count < GRADS; i++) {
     const FsgsGradTensor g = of(i);
     if (g.n == 0) continue;
-    if (turns + turns_of(g, bytes) > MAX_BLOCKS) break;
+    if (turns + turns_of(g) > MAX_TURNS) break;
     const int k = t.count++;
     t.at[k] = {g.grad, g.n << 2 | g.dtype};
     t.start[k] = (uint32_t)turns;
-    turns += turns_of(g, bytes);
+    turns += turns_of(g);
   }
   t.turns = (uint32_t)turns;
   return i;
@@ -664,7 +675,7 @@ template <typename Of> int launch_norm(int n_tensors, Of of, float max_norm, voi
   size_t count = 0;
   GradTable t;
   for (int i = 0; i < n_tensors;) {
-    i = fill_grads(t, i, n_tensors, of, NORM_BYTES);
+    i = fill_grads(t, i, n_tensors, of);
     if (t.count == 0) continue;
     const uint32_t groups = std::min<uint32_t>(t.turns, NORM_GROUPS);
     if ((count + groups) * sizeof(double) > scratch_bytes) return FSGS_ERR_CAPACITY;
@@ -685,9 +696,9 @@ template <typename Of> int launch_norm(int n_tensors, Of of, float max_norm, voi
 template <typename Of> int launch_scale(int n_tensors, Of of, const Bound &bound, hipStream_t stream) {
   GradTable t;
   for (int i = 0; i < n_tensors;) {
-    i = fill_grads(t, i, n_tensors, of, SCALE_BYTES);
+    i = fill_grads(t, i, n_tensors, of);
     if (t.count == 0) continue;
-    hipLaunchKernelGGL(grad_scale_kernel, dim3(t.turns), dim3(THREADS), 0, stream, t, bound);
+    hipLaunchKernelGGL(grad_scale_kernel, dim3(scale_rows(t.turns) * XCDS * 2), dim3(THREADS), 0, stream, t, bound);
     FSGS_HIP(hipGetLastError());
   }
   return FSGS_OK;
@@ -703,7 +714,7 @@ template <typename T, bool MASTER> void launch_step(const Table &t, uint32_t gro
 extern "C" {
 
 size_t fsgs_grad_norm_scratch_bytes(int n_tensors) {
-  // a launch takes 192 tensors, or fewer where they hold over 2^38 bytes: no card holds that 8 times
+  // a launch takes 192 tensors, or fewer where they hold over 2^37 bytes: no card holds that 8 times
   return n_tensors > 0 ? (size_t)((n_tensors + GRADS - 1) / GRADS + 8) * NORM_GROUPS * sizeof(double) : 0;
 }
 
@@ -856,7 +867,7 @@ static int check_grads(int n_tensors, const FsgsGradTensor *grads, bool write) {
   if (!regions.items) return FSGS_ERR_CAPACITY;
   for (int i = 0; i < n_tensors; i++) {
     if (grads[i].n < 0 || !size_of(grads[i].dtype) || (grads[i].n > 0 && !grads[i].grad)) return FSGS_ERR_INVALID;
-    if (grads[i].n > INT64_MAX / 16 || turns_of(grads[i], SCALE_BYTES) > MAX_BLOCKS) return FSGS_ERR_INVALID;
+    if (grads[i].n > INT64_MAX / 16 || turns_of(grads[i]) > MAX_TURNS) return FSGS_ERR_INVALID;
     regions.add(grads[i].grad, grads[i].n * size_of(grads[i].dtype), write);
   }
   return regions.clash() ? FSGS_ERR_INVALID : FSGS_OK;
