@@ -471,7 +471,7 @@ class FusedAdamW(torch.optim.Optimizer):
                 rc = lib.fsgs_adamw_step(n, rows, len(hypers) // _lib.ADAMW_HYPER_BYTES, hypers, b.dtype, b.bits, b.maximize, *limit,
                                          _lib.ptr(scratch), _lib.current_stream())
                 if rc == _lib.FSGS_ERR_INVALID:
-                    raise ValueError("FusedAdamW: two of the tensors of a step share memory (or one has over 2^34 elements)")
+                    raise ValueError("FusedAdamW: two of the tensors of a step share memory (or one has 2^35 elements or more)")
                 _lib.check(rc, "fsgs_adamw_step")
             _lib.host().stepped(b.params, b.states)
         return loss
