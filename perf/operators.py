@@ -12,8 +12,8 @@ boundaries, as programs with one communication bucket hold them.
 8-bit moments: blocks of 128 consecutive elements share one power of two per moment.  The first moment is kept as
 e4m3 codes of m / 2^E, the second as e4m3 codes of sqrt(v) / 2^E; E is the smallest power that brings the block's largest
 value to at most 448.  A value is rounded down or up to a neighbouring code by comparing its remainder with a threshold
-in [0, 1) that belongs to the element and the step (evenly spread over the elements, shifted at each step by a hash of its
-number), so that the mean over steps is unbiased; a second moment that is not zero keeps at least the smallest code."""
+in [0, 1) that belongs to the element and the step (a quasi-random sequence), so that the mean over steps is unbiased; a
+second moment that is not zero keeps at least the smallest code."""
 import math
 import random
 
@@ -26,6 +26,7 @@ POSES = ((4, 0.01), (3, 0.01))
 BETAS = (0.9, 0.999)
 BLOCK = 128
 GOLDEN, ROOT2 = 0x9E3779B9, 0x6A09E667        # 2^32 times the fractions of the golden ratio and of sqrt(2)
+R2_X, R2_Y = 0xC13FA9A9, 0x91E10DA5           # 2^32 / plastic number, 2^32 / its square (the R2 sequence)
 
 
 def listed():
@@ -139,7 +140,7 @@ def _inputs(case, seed):
         else:
             s["m"], s["v"] = [t.clone() for t in cut["m"]], [t.clone() for t in cut["v"]]
     elif case["op"] == "adamw8":
-        enc = [(_encode(m, s["step"], GOLDEN, 0, False), _encode(v.sqrt(), s["step"], ROOT2, 1, True))
+        enc = [(_encode(m, s["step"], GOLDEN, R2_X, False), _encode(v.sqrt(), s["step"], ROOT2, R2_Y, True))
                for m, v in zip(cut["m"], cut["v"])]
         s["mq"], s["rq"] = [e[0][0] for e in enc], [e[1][0] for e in enc]
         s["scales"] = [torch.stack((e[0][1], e[1][1]), 1).contiguous() for e in enc]
@@ -252,19 +253,10 @@ def _step_plain(s):
         torch._foreach_copy_(p, w)
 
 
-def _shift(x):
-    """A hash of 32 bits: two rounds of shift and multiplication, by the fractions of sqrt(3) and sqrt(5)."""
-    x ^= x >> 16
-    x = x * 0xBB67AE85 & 0xFFFFFFFF
-    x ^= x >> 15
-    x = x * 0x3C6EF373 & 0xFFFFFFFF
-    return x ^ x >> 16
-
-
-def _threshold(n, step, phase, which):
-    """Twenty bits of the element's threshold at this step, for the first (0) or second (1) moment."""
+def _threshold(n, step, phase, turn):
+    """Twenty bits of the element's threshold at this step."""
     i = torch.arange(n, device="cuda", dtype=torch.int64)
-    return ((i * phase + _shift(2 * step + which)) & 0xFFFFFFFF) >> 12
+    return ((i * phase + step * turn) & 0xFFFFFFFF) >> 12
 
 
 def _blocks(x):
@@ -276,7 +268,7 @@ def _power(e):
     return (e.to(torch.int32) << 23).view(torch.float32)
 
 
-def _encode(x, step, phase, which, keep):
+def _encode(x, step, phase, turn, keep):
     """(e4m3 codes, one biased exponent for each block) of a flat fp32 tensor."""
     f = _blocks(x)
     fine = torch.isfinite(f)
@@ -284,7 +276,7 @@ def _encode(x, step, phase, which, keep):
     mant, ex = torch.frexp(a.amax(1))
     e = torch.where(mant > 0, (ex - 9 + (mant > 0.875) + 127).clamp(1, 254), torch.ones_like(ex))
     y = a * _power(254 - e)[:, None]
-    u = _blocks(_threshold(x.numel(), step, phase, which))
+    u = _blocks(_threshold(x.numel(), step, phase, turn))
     code = torch.where(y < 2.0 ** -6, (y.double() * 512 + u.double() / 2 ** 20).floor().to(torch.int64),
                        ((y.view(torch.int32).to(torch.int64) + u) >> 20) - 960)
     if keep:
@@ -312,7 +304,7 @@ def _one8(s, w, g, mq, rq, scales, lr):
     m = _decode(mq, scales[:, 0]) * b1 + g * (1 - b1)
     r = (_decode(rq, scales[:, 1]).square() * b2 + g.square() * (1 - b2)).sqrt()
     w.mul_(1 - lr * decay).sub_((lr / (1 - b1 ** t)) * (m / (r / math.sqrt(1 - b2 ** t) + eps)))
-    for codes, column, new in ((mq, 0, _encode(m, t, GOLDEN, 0, False)), (rq, 1, _encode(r, t, ROOT2, 1, True))):
+    for codes, column, new in ((mq, 0, _encode(m, t, GOLDEN, R2_X, False)), (rq, 1, _encode(r, t, ROOT2, R2_Y, True))):
         codes.copy_(new[0])
         scales[:, column] = new[1]
     return _decode(mq, scales[:, 0]).bfloat16(), _decode(rq, scales[:, 1]).square().bfloat16()
@@ -340,7 +332,7 @@ def exact(case, seed):
         w = (s["w"][i] if "w" in s else s["p"][i]).double()
         out["p"].append(w - s["lr"][i] * (mhat / (vhat.sqrt() + case["eps"]) + case["decay"] * w))
         if case["op"] == "adamw8":
-            m, v = _rounded64(m, t, GOLDEN, 0, False), _rounded64(v.sqrt(), t, ROOT2, 1, True) ** 2
+            m, v = _rounded64(m, t, GOLDEN, R2_X, False), _rounded64(v.sqrt(), t, ROOT2, R2_Y, True) ** 2
         out["m"].append(m)
         out["v"].append(v)
     if case["op"] == "adamw":
@@ -365,7 +357,7 @@ def _values64(codes, e):
     return codes.double() * torch.exp2(e.double() - 127).repeat_interleave(BLOCK)[:codes.numel()]
 
 
-def _rounded64(x, step, phase, which, keep):
+def _rounded64(x, step, phase, turn, keep):
     """Every value moved to the code below or above it, by the element's threshold."""
     n = x.numel()
     top = torch.cat((x, x.new_zeros(-n % BLOCK))).view(-1, BLOCK).abs().amax(1)
@@ -377,7 +369,7 @@ def _rounded64(x, step, phase, which, keep):
     grain = torch.exp2(torch.floor(torch.log2(a.clamp(min=2.0 ** -6))) - 3)
     grain = torch.where(a / grain >= 16, grain * 2, torch.where((a / grain < 8) & (grain > 2.0 ** -9), grain / 2, grain))
     i = torch.arange(n, device=x.device)
-    share = torch.floor(((i * phase + _shift(2 * step + which)) % 2 ** 32).double() / 4096) / 2 ** 20
+    share = torch.floor(((i * phase + step * turn) % 2 ** 32).double() / 4096) / 2 ** 20
     near = torch.floor(a / grain + share) * grain
     if keep:
         near = torch.where(x > 0, near.clamp(min=2.0 ** -9), near)
