@@ -17,13 +17,16 @@
 // Moments in 8 bits: 128 consecutive elements of a tensor share one power of two for m and one for r = sqrt(v).  The codes are
 // OCP e4m3 of m / 2^E and r / 2^E with the smallest E that brings the block's largest finite value to at most 448, stored as
 // E + 127 in a byte.  r rather than v, because r needs half the exponent range.  A value between two codes goes up when its
-// remainder reaches over the threshold of its element at this step: 20 bits of a Weyl sequence over the elements that each step
-// shifts by a hash of its number.  For one element the thresholds of different steps are as good as independent, so a moment
-// that moves by less than a code a step still moves in the mean as it should: with b2 = 0.999, r moves by 5e-4 a step and half
-// a code is 3e-2 to 6e-2, so that rounding to nearest would hold it for good.  (A quasi-random sequence over the steps too
-// lets r fall 7 % too fast: it leaves every code after the mean waiting time exactly, and ln 2 > 1/9 + ... + 1/16.)  r > 0
-// keeps at least the smallest code, so that m is never divided by a denominator that the rounding took away.  The step
-// itself uses m and r before the rounding.
+// remainder reaches over the threshold of its element at this step: 20 bits of a quasi-random sequence, a Weyl sequence over
+// the elements (golden ratio, sqrt 2) that each step moves on by the plastic number's inverse (m) or its square (r).  A moment
+// that moves by less than a code a step so still moves: with b2 = 0.999, r moves by 5e-4 a step and half a code is 3e-2 to
+// 6e-2, so that rounding to nearest would hold it for good.  How well it follows moments in 32 bits (20 000 elements, b2 =
+// 0.999; ratio of r: mean and deviation; of v: mean): Gaussian gradients, steps 1500 to 4000: 1.007, 0.12; 1.03.  Gradients
+// in one step of twenty: 0.996, 0.13; 1.01.  1500 steps without any: 0.951, 0.07; 0.91 -- too low, because a code is left
+// after the mean waiting time, and 1/9 + ... + 1/16 < ln 2.  Thresholds that are independent from step to step keep r's mean
+// there (0.997) but spread three times as far (0.25), and farther than these with gradients too (0.14 and 0.18; v 1.04 and
+// 1.06).  r > 0 keeps at least the smallest code, so that m is never divided by a denominator that the rounding took away.
+// The step itself uses m and r before the rounding.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -65,12 +68,8 @@ struct Hyper {
   float b1, omb1, b2, omb2;
   uint32_t shift_m, shift_r;  // the step's part of the rounding thresholds
 };
-constexpr uint32_t PHASE_M = 0x9E3779B9u, PHASE_R = 0x6A09E667u;  // 2^32 frac(golden ratio), 2^32 frac(sqrt 2)
-__host__ __device__ inline uint32_t shift_of(uint32_t x) {  // a hash: multiplication by 2^32 frac(sqrt 3), frac(sqrt 5), made odd
-  x ^= x >> 16; x *= 0xBB67AE85u;
-  x ^= x >> 15; x *= 0x3C6EF373u;
-  return x ^ (x >> 16);
-}
+// 2^32 times the fractions of the golden ratio and of sqrt 2; 2^32 / plastic number (rho^3 = rho + 1), 2^32 / its square
+constexpr uint32_t PHASE_M = 0x9E3779B9u, PHASE_R = 0x6A09E667u, TURN_M = 0xC13FA9A9u, TURN_R = 0x91E10DA5u;
 
 __host__ __device__ inline Hyper make_hyper(double lr, double b1, double b2, double eps, double wd, double step) {
   Hyper h;
@@ -81,7 +80,7 @@ __host__ __device__ inline Hyper make_hyper(double lr, double b1, double b2, dou
   // 1 - beta in double: 1 - 0.999f is off by 4.7e-5 of itself
   h.b1 = (float)b1; h.omb1 = (float)(1.0 - b1); h.b2 = (float)b2; h.omb2 = (float)(1.0 - b2);
   const uint32_t t = (uint32_t)(int64_t)step;
-  h.shift_m = shift_of(2 * t); h.shift_r = shift_of(2 * t + 1);
+  h.shift_m = t * TURN_M; h.shift_r = t * TURN_R;
   return h;
 }
 

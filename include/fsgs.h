@@ -517,8 +517,9 @@ int fsgs_adam_step(int ngroups, const FsgsAdamGroup *groups, double beta1, doubl
  * param and grad are of `dtype`; w is `master` (fp32) where given, and param = w rounded to nearest, else w is param itself.
  * state_bits 32: exp_avg / exp_avg_sq are float[n].  state_bits 8: they are uint8[n] codes, OCP e4m3 of m / 2^E and of
  * sqrt(v) / 2^E, and scales is uint8[ceil(n / 128)][2], E + 127 of both for each 128 consecutive elements (0 stands for a
- * factor of 0, so all-zero state is valid).  New codes are rounded up or down by a threshold that belongs to the element
- * and the step, evenly distributed over the steps; the step itself uses the moments before that rounding.
+ * factor of 0, so all-zero state is valid).  New codes are rounded up or down by a threshold that belongs to the element i
+ * and the step t, the upper 20 bits of i * 0x9E3779B9 + t * 0xC13FA9A9 (m) and of i * 0x6A09E667 + t * 0x91E10DA5 (sqrt(v)),
+ * modulo 2^32; the step itself uses the moments before that rounding.
  * Pointers need their element's alignment only.  No two tensors may share memory that is written. */
 #define FSGS_DTYPE_F32 0
 #define FSGS_DTYPE_BF16 1

@@ -23,7 +23,16 @@ def _has_gpu():
         return False
 
 
+# Tests whose expected values are those of another rounding rule than the one that 8-bit moments are defined by (include/fsgs.h,
+# fsgs_adamw_step): thresholds hashed from the step, and the mean that such thresholds keep without gradients.  They stay as they
+# are, run, and have to fail; tests/test_adamw8_rounding_gpu.py holds the same checks with the values of the definition.
+OTHER_ROUNDING = {"test_steps_in_8_bits", "test_the_rounding_is_unbiased_over_steps", "test_offsets_over_32_bits"}
+
+
 def pytest_collection_modifyitems(config, items):
+    for item in items:
+        if item.module.__name__.rsplit(".", 1)[-1] == "test_adamw_gpu" and item.function.__name__ in OTHER_ROUNDING:
+            item.add_marker(pytest.mark.xfail(strict=True, raises=AssertionError, reason="expects thresholds hashed from the step"))
     if _has_gpu():
         return
     skip = pytest.mark.skip(reason="no GPU in this container")
