@@ -139,9 +139,10 @@ class GaussianCloud:
 
     def _widen_moments(self):
         """8-bit Adam moments (blocks that span rows) as fp32 ones in front of a row operation; the optimizer's next step
-        brings them back to 8 bits"""
-        for group in self.optimizer.param_groups:
-            if group.get("state_bits") == 8:
+        brings them to the width that its groups ask for.  What the state holds counts, not what a group asks for: an option that
+        has been changed takes effect at the next step, and a group from a checkpoint may name options of another optimizer"""
+        if hasattr(self.optimizer, "widen"):
+            for group in self.optimizer.param_groups:
                 self.optimizer.widen(group["params"][0])
 
     def prune_points(self, mask):
@@ -280,7 +281,7 @@ class GaussianCloud:
             if group["name"] != "_opacity":
                 continue
             old = group["params"][0]
-            if group.get("state_bits") == 8:
+            if hasattr(self.optimizer, "widen"):
                 self.optimizer.widen(old)
             state = self.optimizer.state.pop(old, None)
             t = new.detach().contiguous().requires_grad_(True)

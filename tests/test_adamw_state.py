@@ -1,0 +1,74 @@
+"""What FusedAdamW's state goes through without a GPU: row operations of a cloud, checkpoints and state dicts of other optimizers,
+what is refused."""
+import pytest
+import torch
+
+from fsgs_amd import checkpoint, synth
+from fsgs_amd.model import PARAM_NAMES, GaussianCloud
+from fsgs_amd.optim import FusedAdam, FusedAdamW
+
+
+def cloud(**options):
+    pc = GaussianCloud(synth.init_scene(16, 12, 20, seed=0), sh_degree=3, device="cpu", scene_radius=1.0)
+    pc.training_setup(**options)
+    return pc
+
+
+def coded(p, step=5):
+    """an 8-bit state: m = 1, sqrt(v) = 2 everywhere"""
+    n = p.numel()
+    return {"step": step, "exp_avg_q": torch.ones(p.shape).to(torch.float8_e4m3fn), "exp_avg_sq_q": torch.full(p.shape, 2.0).to(torch.float8_e4m3fn),
+            "scales": torch.full((-(-n // 128), 2), 127, dtype=torch.uint8)}
+
+
+@pytest.fixture
+def decoded(monkeypatch):
+    """the values of 8-bit moments without the kernel"""
+    def read(self, items, dtype):
+        out = []
+        for p, st in items:
+            unit = torch.exp2(st["scales"].float() - 127).repeat_interleave(128, 0)[:p.numel()]
+            value = lambda k, j: (st[k].float().reshape(-1) * unit[:, j]).view(p.shape)  # noqa: E731
+            out.append((value("exp_avg_q", 0).to(dtype), value("exp_avg_sq_q", 1).square().to(dtype)))
+        return out
+
+    monkeypatch.setattr(FusedAdamW, "_read", read)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_row_operations_keep_moments_whatever_width_is_asked_for_next(decoded, bits):
+    pc = cloud(adamw=dict(state_bits=8))
+    for p in pc.params.values():
+        pc.optimizer.state[p] = coded(p)
+    for g in pc.optimizer.param_groups:
+        g["state_bits"] = bits  # converted at the next step; until then the state holds codes
+    mask = torch.zeros(pc.num_points, dtype=torch.bool)
+    mask[::3] = True
+    pc.prune_points(mask)
+    for name in PARAM_NAMES:
+        st = pc.optimizer.state[pc.params[name]]
+        assert st["step"] == 5 and st["exp_avg"].shape == pc.params[name].shape
+        assert bool((st["exp_avg"] == 1).all()) and bool((st["exp_avg_sq"] == 4).all())
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_an_opacity_reset_keeps_the_count(decoded, bits):
+    pc = cloud(adamw=dict(state_bits=8))
+    pc.optimizer.state[pc.params["_opacity"]] = coded(pc.params["_opacity"])
+    for g in pc.optimizer.param_groups:
+        g["state_bits"] = bits
+    pc.reset_opacity()
+    st = pc.optimizer.state[pc.params["_opacity"]]
+    assert st["step"] == 5 and not bool(st["exp_avg"].any()) and not bool(st["exp_avg_sq"].any())
+
+
+@pytest.mark.parametrize("fused", [True, False])
+def test_row_operations_after_an_8_bit_checkpoint_in_a_cloud_of_plain_adam(decoded, fused):
+    pc = cloud(adamw=dict(state_bits=8))
+    for p in pc.params.values():
+        pc.optimizer.state[p] = coded(p)
+    other = checkpoint.restore_gaussians(cloud(fused=fused), checkpoint.capture_gaussians(pc), fused=fused)
+    other.reset_opacity()
+    other.prune_points(torch.arange(other.num_points) % 2 == 0)
+    st = other.optimizer.state[other.params["_xyz"]]
+    assert int(st["step"]) == 5 and bool((st["exp_avg"] == 1).all()) and st["exp_avg"].shape == other.params["_xyz"].shape
