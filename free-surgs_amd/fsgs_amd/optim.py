@@ -133,7 +133,8 @@ def _grads_of(params, who):
     if fast is not None:
         table, index, norm, scratch = fast
         return _Grads(torch.device("cuda", index) if index >= 0 else None, table, norm, scratch)
-    return _grads_from([p.grad for p in params if p.grad is not None], who)
+    grads = [p.grad for p in params if p.grad is not None]
+    return _grads_from(grads, who) if grads else _Grads(None, b"", None, None)
 
 
 @torch.no_grad()

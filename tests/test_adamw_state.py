@@ -5,7 +5,7 @@ import torch
 
 from fsgs_amd import checkpoint, synth
 from fsgs_amd.model import PARAM_NAMES, GaussianCloud
-from fsgs_amd.optim import FusedAdam, FusedAdamW
+from fsgs_amd.optim import FusedAdamW, clip_grad_norm_
 
 
 def cloud(**options):
@@ -72,3 +72,15 @@ def test_row_operations_after_an_8_bit_checkpoint_in_a_cloud_of_plain_adam(decod
     other.prune_points(torch.arange(other.num_points) % 2 == 0)
     st = other.optimizer.state[other.params["_xyz"]]
     assert int(st["step"]) == 5 and bool((st["exp_avg"] == 1).all()) and st["exp_avg"].shape == other.params["_xyz"].shape
+
+
+def test_clipping_parameters_of_a_subclass_that_have_no_gradients():
+    class Weight(torch.nn.Parameter):
+        pass
+
+    for params in (Weight(torch.ones(3)), [Weight(torch.ones(3)), torch.ones(2, requires_grad=True)], (p for p in [Weight(torch.ones(1))])):
+        assert float(clip_grad_norm_(params, 1.0)) == 0.0
+    w = Weight(torch.ones(3))
+    w.grad = torch.ones(3)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        clip_grad_norm_(w, 1.0)
