@@ -24,6 +24,10 @@ _TORCH_ADAM_GROUP_DEFAULTS = dict(weight_decay=0, amsgrad=False, maximize=False,
                                   differentiable=False, fused=None, decoupled_weight_decay=False)
 
 
+# FusedAdamW's options of how state is held and counted: a matter of the run, not of the checkpoint
+_STORAGE = ("state_bits", "master_weights", "capturable")
+
+
 def portable_state_dict(optimizer):
     """optimizer.state_dict() as torch.optim.Adam would have written it: every `step` a 0-d float32 CPU tensor and
     every param_group carrying the keys torch's Adam reads (FusedAdam's own defaults are lr / betas / eps only)."""
@@ -31,6 +35,9 @@ def portable_state_dict(optimizer):
     if hasattr(optimizer, "widen"):  # FusedAdamW: moments as values whatever their width, in entries of their own
         for packed, group in zip(sd["param_groups"], optimizer.param_groups):
             packed["decoupled_weight_decay"] = True
+            for k in _STORAGE:  # how this run holds its state, not what the file holds
+                packed.pop(k, None)
+            packed["lr"] = float(packed["lr"])  # a captured step's may be a tensor on the device
             for i, p in zip(packed["params"], group["params"]):
                 if i in sd["state"]:
                     sd["state"][i] = optimizer.wide_state(p)
@@ -53,7 +60,9 @@ def capture_gaussians(pc):
 
 def restore_gaussians(pc, model_args, opt=OptimizationParams, eps=1e-15, fused=True):
     """GaussianModel.restore (scene/gaussian_model.py:102-116): install the tensors, rebuild the optimizer with the
-    mapping learning rates, load the Adam state.  Anything holding the old tensors (a FastStepper) must be rebuilt."""
+    mapping learning rates, load the Adam state.  Anything holding the old tensors (a FastStepper) must be rebuilt.
+    Learning rates are the file's.  A cloud with options for FusedAdamW (training_setup(adamw=...)) keeps those that it names, and
+    its own width of the moments, masters and capturable; the file has the rest (a weight decay, betas, eps not named)."""
     if len(model_args) != 12:
         raise ValueError("expected the 12-tuple of GaussianModel.capture(), got %d entries" % len(model_args))
     dev = pc.params["_xyz"].device
@@ -81,6 +90,11 @@ def restore_gaussians(pc, model_args, opt=OptimizationParams, eps=1e-15, fused=T
         "param_groups": sd["param_groups"],
         "state": {k: {n: (v.detach().clone() if torch.is_tensor(v) else v) for n, v in st.items()}
                   for k, st in sd["state"].items()}})
+    if pc.adamw is not None:
+        own = {k: pc.optimizer.defaults[k] for k in _STORAGE}
+        own.update((k, v) for k, v in pc.adamw.items() if k in pc.optimizer.defaults and k != "lr")
+        for group in pc.optimizer.param_groups:
+            group.update(own)
     return pc
 
 

@@ -85,7 +85,8 @@ class GaussianCloud:
         """Adam with the reference's per-group learning rates (scene/gaussian_model.py:382-409).
         fused=True: one HIP launch per step (fsgs_amd.optim.FusedAdam); False: torch.optim.Adam.
         adamw: a dict of options for fsgs_amd.optim.FusedAdamW instead (weight_decay -- 0 unless given --, state_bits=8,
-        max_grad_norm, betas, ...), kept for the optimizers that initialize_optimizer and a restored checkpoint build;
+        max_grad_norm, betas, ...), kept for the optimizers that initialize_optimizer and a restored checkpoint build (the
+        options named here go before those of the checkpoint; learning rates are the checkpoint's);
         {} is Adam's arithmetic with FusedAdamW's state.  The step driver then runs its unfused optimizer step."""
         self.adamw = None if adamw is None else dict(adamw)
         lr = {"_xyz": opt.position_lr_init * self.spatial_lr_scale, "_features_dc": opt.feature_lr,

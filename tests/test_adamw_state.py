@@ -84,3 +84,46 @@ def test_clipping_parameters_of_a_subclass_that_have_no_gradients():
     w.grad = torch.ones(3)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         clip_grad_norm_(w, 1.0)
+
+
+def saved(**options):
+    pc = cloud(**options)
+    for i, g in enumerate(pc.optimizer.param_groups):
+        g["lr"] = 1e-4 * (i + 1)
+    for p in pc.params.values():
+        if options.get("adamw", {}).get("state_bits") == 8:
+            pc.optimizer.state[p] = coded(p)
+        else:
+            pc.optimizer.state[p] = {"step": 5, "exp_avg": torch.ones_like(p), "exp_avg_sq": torch.full_like(p, 4.0)}
+    return checkpoint.capture_gaussians(pc)
+
+
+@pytest.mark.parametrize("file,asked,want", [
+    # the options that a cloud names go before the file's ...
+    (dict(), dict(weight_decay=0.01, betas=(0.9, 0.99), eps=1e-8, state_bits=8),
+     dict(weight_decay=0.01, betas=(0.9, 0.99), eps=1e-8, state_bits=8)),
+    (dict(fused=False), dict(weight_decay=0.01, maximize=True), dict(weight_decay=0.01, maximize=True, state_bits=32)),
+    (dict(adamw=dict(state_bits=8, weight_decay=0.1)), dict(state_bits=32, weight_decay=0.0), dict(state_bits=32, weight_decay=0.0)),
+    # ... those that it does not name are the file's, but for how state is held
+    (dict(adamw=dict(weight_decay=0.1, betas=(0.8, 0.99), eps=1e-6)), dict(state_bits=8),
+     dict(weight_decay=0.1, betas=(0.8, 0.99), eps=1e-6, state_bits=8)),
+    (dict(adamw=dict(state_bits=8, master_weights=True, capturable=True)), dict(),
+     dict(state_bits=32, master_weights=False, capturable=False, eps=1e-15)),
+])
+def test_a_restored_cloud_has_the_options_that_it_names(decoded, file, asked, want):
+    pc = cloud(adamw={**asked, "lr": 7.0, "max_grad_norm": 2.0})
+    checkpoint.restore_gaussians(pc, saved(**file))
+    assert isinstance(pc.optimizer, FusedAdamW) and pc.optimizer.max_grad_norm == 2.0
+    for i, g in enumerate(pc.optimizer.param_groups):
+        assert {k: g[k] for k in want} == want and g["lr"] == 1e-4 * (i + 1) and "max_grad_norm" not in g
+    st = pc.optimizer.state[pc.params["_xyz"]]
+    assert int(st["step"]) == 5 and bool((st["exp_avg"] == 1).all()) and bool((st["exp_avg_sq"] == 4).all())
+
+
+def test_a_checkpoint_says_nothing_of_how_its_run_held_the_state(decoded):
+    pc = cloud(adamw=dict(state_bits=8, master_weights=True, capturable=True))
+    pc.optimizer.param_groups[0]["lr"] = torch.tensor(0.25)
+    groups = checkpoint.capture_gaussians(pc)[10]["param_groups"]
+    assert all("state_bits" not in g and "master_weights" not in g and g["capturable"] is False for g in groups)
+    assert type(groups[0]["lr"]) is float and groups[0]["lr"] == 0.25
+    assert all(g["state_bits"] == 8 and g["capturable"] for g in pc.optimizer.param_groups)  # the run's own stay

@@ -60,3 +60,28 @@ def test_a_width_changed_in_front_of_a_row_operation(before, after, op):
     for p in pc.params.values():
         st = pc.optimizer.state[p]
         assert st["step"] == 3 and ("exp_avg_q" in st) == (after == 8) and ("exp_avg" in st) == (after == 32)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_cloud_of_the_other_width_and_decay_restores(bits, tmp_path):
+    pc = stepped(cloud(state_bits=bits, weight_decay=0.1))
+    torch.save(checkpoint.capture_gaussians(pc), os.path.join(str(tmp_path), "cloud.pth"))
+    saved = torch.load(os.path.join(str(tmp_path), "cloud.pth"), weights_only=True)
+    other = checkpoint.restore_gaussians(cloud(state_bits=40 - bits, weight_decay=0.0, max_grad_norm=5.0), saved)
+    wide = dict(zip(PARAM_NAMES, other.optimizer.moments()))
+    for (m, v), (m2, v2) in zip(pc.optimizer.moments(), wide.values()):
+        assert torch.equal(m, m2) and torch.equal(v, v2)
+    before = {k: p.detach().clone() for k, p in other.params.items()}
+    for p in other.params.values():
+        p.grad = torch.zeros_like(p)
+    other.optimizer.step()
+    for g in other.optimizer.param_groups:
+        p, name = g["params"][0], g["name"]
+        st = other.optimizer.state[p]
+        assert g["state_bits"] == 40 - bits and st["step"] == 3 and ("exp_avg_q" in st) == (bits == 32) and ("exp_avg" in st) == (bits == 8)
+        m, v = (0.9 * wide[name][0].double(), 0.999 * wide[name][1].double())
+        if bits == 32:  # the moments went into codes before the step: 1/16 of a value, or half of the smallest code
+            continue
+        u = g["lr"] / (1 - 0.9 ** 3) * m / (v.sqrt() / math.sqrt(1 - 0.999 ** 3) + g["eps"])
+        want = before[name].double() - u  # no decay: w and its sum 2 roundings, the step 16
+        assert bool(((p.detach().double() - want).abs() <= 2.0 ** -24 * (2 * want.abs() + 16 * u.abs())).all())
