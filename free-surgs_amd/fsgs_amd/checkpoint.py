@@ -62,9 +62,15 @@ def restore_gaussians(pc, model_args, opt=OptimizationParams, eps=1e-15, fused=T
     """GaussianModel.restore (scene/gaussian_model.py:102-116): install the tensors, rebuild the optimizer with the
     mapping learning rates, load the Adam state.  Anything holding the old tensors (a FastStepper) must be rebuilt.
     Learning rates are the file's.  A cloud with options for FusedAdamW (training_setup(adamw=...)) keeps those that it names, and
-    its own width of the moments, masters and capturable; the file has the rest (a weight decay, betas, eps not named)."""
+    its own width of the moments, masters and capturable; the file has the rest (a weight decay, betas, eps not named).
+    FusedAdam neither decays nor ascends: a file whose run did (AdamW's) needs such a cloud, adamw={} at least, or fused=False."""
     if len(model_args) != 12:
         raise ValueError("expected the 12-tuple of GaussianModel.capture(), got %d entries" % len(model_args))
+    if fused and getattr(pc, "adamw", None) is None:
+        for g in model_args[10]["param_groups"]:
+            if g.get("decoupled_weight_decay") and (g.get("weight_decay") or g.get("maximize")):
+                raise ValueError("the checkpoint's optimizer has weight_decay=%r, maximize=%r (AdamW), which FusedAdam would ignore: "
+                                 "call training_setup(adamw={}) on the cloud first" % (g.get("weight_decay"), g.get("maximize")))
     dev = pc.params["_xyz"].device
     # always a COPY: a tuple captured from a live model (not read from disk) must not end up sharing parameter or
     # moment storage with the model it is restored into

@@ -127,3 +127,18 @@ def test_a_checkpoint_says_nothing_of_how_its_run_held_the_state(decoded):
     assert all("state_bits" not in g and "master_weights" not in g and g["capturable"] is False for g in groups)
     assert type(groups[0]["lr"]) is float and groups[0]["lr"] == 0.25
     assert all(g["state_bits"] == 8 and g["capturable"] for g in pc.optimizer.param_groups)  # the run's own stay
+
+
+@pytest.mark.parametrize("options", [dict(weight_decay=0.1), dict(maximize=True)])
+def test_a_checkpoint_whose_run_decayed_or_ascended_is_not_continued_without(options):
+    file = saved(adamw=options)
+    pc = cloud()
+    before, optimizer = dict(pc.params), pc.optimizer
+    with pytest.raises(ValueError, match=list(options)[0]):
+        checkpoint.restore_gaussians(pc, file)
+    assert all(pc.params[k] is before[k] for k in before) and pc.optimizer is optimizer
+    for ready in (cloud(adamw={}), cloud(fused=False)):
+        checkpoint.restore_gaussians(ready, file, fused=ready.adamw is not None)
+        assert all({k: g[k] for k in options} == options for g in ready.optimizer.param_groups)
+    assert ready.optimizer.param_groups[0]["decoupled_weight_decay"] is True
+    checkpoint.restore_gaussians(cloud(), saved(adamw=dict(weight_decay=0.0)))  # nothing is lost
