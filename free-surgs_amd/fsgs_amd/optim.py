@@ -428,7 +428,16 @@ class FusedAdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """as torch's, but every entry keeps its own type (torch casts floating state to the parameter's)"""
-        super().load_state_dict(state_dict)
+        taken = []
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, sd: taken.append(sd)),  # the last: what the others made of it
+                 self.register_load_state_dict_post_hook(lambda _: self._keep_types(taken[-1]), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
+
+    def _keep_types(self, state_dict):
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         mine = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, mine):

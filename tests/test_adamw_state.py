@@ -142,3 +142,32 @@ def test_a_checkpoint_whose_run_decayed_or_ascended_is_not_continued_without(opt
         assert all({k: g[k] for k in options} == options for g in ready.optimizer.param_groups)
     assert ready.optimizer.param_groups[0]["decoupled_weight_decay"] is True
     checkpoint.restore_gaussians(cloud(), saved(adamw=dict(weight_decay=0.0)))  # nothing is lost
+
+
+def adam_state(p, dtype=torch.float32, step=3):
+    return {"step": step, "exp_avg": torch.full(p.shape, 2.0, dtype=dtype), "exp_avg_sq": torch.full(p.shape, 3.0, dtype=dtype)}
+
+
+def test_hooks_of_a_load_have_the_last_word():
+    p = torch.ones(2, 3, dtype=torch.bfloat16, requires_grad=True)
+    opt = FusedAdamW([p])
+    opt.state[p] = adam_state(p)
+    other = FusedAdamW([p.detach().clone().requires_grad_(True)])
+    q = other.param_groups[0]["params"][0]
+
+    def another(_, sd):
+        return {**sd, "state": {0: {"step": 9, "exp_avg": torch.full((2, 3), 1.001), "exp_avg_sq": torch.full((2, 3), 5.0)}}}
+
+    def after(o):
+        assert o.state[q]["exp_avg"].dtype == torch.float32  # a hook sees what has been loaded
+        o.state[q]["exp_avg_sq"] = torch.full((2, 3), 7.0)
+
+    other.register_load_state_dict_pre_hook(another)
+    other.register_load_state_dict_post_hook(after)
+    for _ in range(2):
+        other.load_state_dict(opt.state_dict())
+        st = other.state[q]
+        assert st["step"] == 9 and bool((st["exp_avg"] == torch.tensor(1.001)).all()) and bool((st["exp_avg_sq"] == 7).all())
+    with pytest.raises(ValueError):
+        other.load_state_dict({"state": {}, "param_groups": []})
+    assert len(other._optimizer_load_state_dict_pre_hooks) == len(other._optimizer_load_state_dict_post_hooks) == 1
