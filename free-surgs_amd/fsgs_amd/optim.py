@@ -427,7 +427,8 @@ class FusedAdamW(torch.optim.Optimizer):
         self._ready(p, st, group)
 
     def load_state_dict(self, state_dict):
-        """as torch's, but every entry keeps its own type (torch casts floating state to the parameter's)"""
+        """as torch's, but every entry keeps its own type (torch casts floating state to the parameter's), and moments and masters
+        become float32 in the parameter's layout, whatever floating type another optimizer held them in"""
         taken = []
         hooks = (self.register_load_state_dict_pre_hook(lambda _, sd: taken.append(sd)),  # the last: what the others made of it
                  self.register_load_state_dict_post_hook(lambda _: self._keep_types(taken[-1]), prepend=True))
@@ -443,7 +444,7 @@ class FusedAdamW(torch.optim.Optimizer):
         for i, p in zip(saved, mine):
             for k, v in state_dict["state"].get(i, {}).items():
                 if torch.is_tensor(v) and k != "step":
-                    if v.dtype == _F32 and v.shape == p.shape:  # whatever layout it was saved in
+                    if k in ("exp_avg", "exp_avg_sq", "master") and v.is_floating_point() and v.shape == p.shape:
                         self.state[p][k] = torch.empty_like(p, dtype=_F32, memory_format=torch.preserve_format,
                                                             requires_grad=False).copy_(v.detach())
                     else:

@@ -171,3 +171,23 @@ def test_hooks_of_a_load_have_the_last_word():
     with pytest.raises(ValueError):
         other.load_state_dict({"state": {}, "param_groups": []})
     assert len(other._optimizer_load_state_dict_pre_hooks) == len(other._optimizer_load_state_dict_post_hooks) == 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_moments_of_any_floating_type_load_as_float32(dtype, bits):
+    """torch's AdamW holds the moments of 16-bit parameters in 16 bits"""
+    p = torch.ones(4, 3, dtype=dtype, requires_grad=True)
+    p.grad = torch.full((4, 3), 0.25, dtype=dtype)
+    theirs = torch.optim.AdamW([p])
+    theirs.step()
+    assert theirs.state[p]["exp_avg"].dtype == dtype
+    q = torch.ones(3, 4, dtype=torch.bfloat16).t().requires_grad_(True)  # another order of dimensions
+    opt = FusedAdamW([q], state_bits=bits, master_weights=True)
+    sd = theirs.state_dict()
+    sd["state"][0]["master"] = torch.full((4, 3), 1.5, dtype=dtype)
+    opt.load_state_dict(sd)
+    st = opt.state[q]
+    for k, v in (("exp_avg", theirs.state[p]["exp_avg"]), ("exp_avg_sq", theirs.state[p]["exp_avg_sq"]), ("master", sd["state"][0]["master"])):
+        assert st[k].dtype == torch.float32 and st[k].stride() == q.stride() and torch.equal(st[k], v.float()) and not st[k].requires_grad
+    assert int(st["step"]) == 1 and opt._state_tensors(q, st, 32)[0] is st["exp_avg"]

@@ -85,3 +85,32 @@ def test_a_cloud_of_the_other_width_and_decay_restores(bits, tmp_path):
         u = g["lr"] / (1 - 0.9 ** 3) * m / (v.sqrt() / math.sqrt(1 - 0.999 ** 3) + g["eps"])
         want = before[name].double() - u  # no decay: w and its sum 2 roundings, the step 16
         assert bool(((p.detach().double() - want).abs() <= 2.0 ** -24 * (2 * want.abs() + 16 * u.abs())).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_states_of_torchs_adamw_go_on(dtype, bits):
+    """the same gradients once more: 32-bit moments move as the formula says from the 16-bit ones that torch held"""
+    ps, gs = make([300, 5], dtype, seed=8)
+    theirs = torch.optim.AdamW(ps, lr=1e-2)
+    for p, g in zip(ps, gs):
+        p.grad = g
+    theirs.step()
+    qs = [p.detach().clone().requires_grad_(True) for p in ps]
+    opt = FusedAdamW(qs, state_bits=bits)
+    opt.load_state_dict(theirs.state_dict())
+    for g in opt.param_groups:
+        assert g["state_bits"] == bits and g["lr"] == 1e-2 and g["weight_decay"] == 1e-2
+    for q, g in zip(qs, gs):
+        q.grad = g
+    opt.step()
+    for p, q, g, (m, v) in zip(ps, qs, gs, opt.moments()):
+        want = 0.9 * theirs.state[p]["exp_avg"].double() + 0.1 * g.double()
+        size = 0.9 * theirs.state[p]["exp_avg"].double().abs() + 0.1 * g.double().abs()
+        assert opt.state[q]["step"] == 2
+        if bits == 32:
+            assert bool(((m.double() - want).abs() <= 5 * 2.0 ** -24 * size + 2.0 ** -149).all())
+        # torch's own fp16 step leaves infinities and NaN: eps = 1e-8 and 1e-3 g^2 for |g| < 5e-3 are under 2^-25, half of the
+        # smallest fp16, so that it divides by zero.  They stay, and the step adds none.
+        fine = torch.isfinite(p)
+        assert bool(torch.isfinite(v).all()) and torch.equal(torch.isfinite(q), fine) and not torch.equal(p[fine], q[fine])
