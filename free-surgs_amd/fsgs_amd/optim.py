@@ -244,6 +244,7 @@ class FusedAdamW(torch.optim.Optimizer):
         group = self.param_groups[-1]
         try:
             self._scalars(group)
+            self._no_amsgrad(group)
             if len({id(p) for p in group["params"]}) != len(group["params"]):
                 raise ValueError("FusedAdamW: a parameter is given twice in one group")
             for p in group["params"]:
@@ -263,6 +264,11 @@ class FusedAdamW(torch.optim.Optimizer):
         for group in self.param_groups:  # groups saved by another Adam
             for k, v in self.defaults.items():
                 group.setdefault(k, v)
+
+    @staticmethod
+    def _no_amsgrad(group):
+        if group.get("amsgrad"):
+            raise ValueError("FusedAdamW: amsgrad is not supported")
 
     @staticmethod
     def _scalars(group):
@@ -430,7 +436,13 @@ class FusedAdamW(torch.optim.Optimizer):
         """as torch's, but every entry keeps its own type (torch casts floating state to the parameter's), and moments and masters
         become float32 in the parameter's layout, whatever floating type another optimizer held them in"""
         taken = []
-        hooks = (self.register_load_state_dict_pre_hook(lambda _, sd: taken.append(sd)),  # the last: what the others made of it
+
+        def take(_, sd):  # the last of these hooks: what the others made of it
+            for group in sd["param_groups"]:
+                self._no_amsgrad(group)
+            taken.append(sd)
+
+        hooks = (self.register_load_state_dict_pre_hook(take),
                  self.register_load_state_dict_post_hook(lambda _: self._keep_types(taken[-1]), prepend=True))
         try:
             super().load_state_dict(state_dict)

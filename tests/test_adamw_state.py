@@ -191,3 +191,23 @@ def test_moments_of_any_floating_type_load_as_float32(dtype, bits):
     for k, v in (("exp_avg", theirs.state[p]["exp_avg"]), ("exp_avg_sq", theirs.state[p]["exp_avg_sq"]), ("master", sd["state"][0]["master"])):
         assert st[k].dtype == torch.float32 and st[k].stride() == q.stride() and torch.equal(st[k], v.float()) and not st[k].requires_grad
     assert int(st["step"]) == 1 and opt._state_tensors(q, st, 32)[0] is st["exp_avg"]
+
+
+def test_amsgrad_is_refused_and_changes_nothing():
+    p, q = torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    p.grad = torch.ones(3)
+    theirs = torch.optim.AdamW([p], amsgrad=True, lr=0.5)
+    theirs.step()
+    opt = FusedAdamW([q], lr=0.25)
+    opt.state[q] = adam_state(q)
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.load_state_dict(theirs.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.25 and opt.state[q]["step"] == 3 and not opt._optimizer_load_state_dict_pre_hooks
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.add_param_group({"params": [torch.ones(2, requires_grad=True)], "amsgrad": True})
+    assert len(opt.param_groups) == 1
+    with pytest.raises(ValueError, match="amsgrad"):
+        FusedAdamW([{"params": [q], "amsgrad": True}])
+    theirs.param_groups[0]["amsgrad"] = False
+    opt.load_state_dict(theirs.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5 and int(opt.state[q]["step"]) == 1
