@@ -455,7 +455,9 @@ class FusedAdamW(torch.optim.Optimizer):
         mine = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, mine):
             for k, v in state_dict["state"].get(i, {}).items():
-                if torch.is_tensor(v) and k != "step":
+                if torch.is_tensor(v) and k == "step":  # torch has moved it where it belongs, and may have kept the very tensor
+                    self.state[p][k] = self.state[p][k].clone()
+                elif torch.is_tensor(v):
                     if k in ("exp_avg", "exp_avg_sq", "master") and v.is_floating_point() and v.shape == p.shape:
                         self.state[p][k] = torch.empty_like(p, dtype=_F32, memory_format=torch.preserve_format,
                                                             requires_grad=False).copy_(v.detach())

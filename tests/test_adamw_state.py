@@ -211,3 +211,16 @@ def test_amsgrad_is_refused_and_changes_nothing():
     theirs.param_groups[0]["amsgrad"] = False
     opt.load_state_dict(theirs.state_dict())
     assert opt.param_groups[0]["lr"] == 0.5 and int(opt.state[q]["step"]) == 1
+
+
+@pytest.mark.parametrize("capturable", [True, False])
+def test_a_loaded_state_shares_nothing_with_the_other_optimizer(capturable):
+    p = torch.ones(3, requires_grad=True)
+    opt = FusedAdamW([p], capturable=capturable)
+    opt.state[p] = {**adam_state(p, step=torch.tensor(4.0)), **coded(p, step=torch.tensor(4.0)), "master": torch.ones(3)}
+    other = FusedAdamW([p.detach().clone().requires_grad_(True)], capturable=capturable)
+    other.load_state_dict(opt.state_dict())
+    st = other.state[other.param_groups[0]["params"][0]]
+    assert float(st["step"]) == 4.0 and all(st[k].data_ptr() != v.data_ptr() for k, v in opt.state[p].items())
+    opt.state[p]["step"].add_(1.0)
+    assert float(st["step"]) == 4.0

@@ -114,3 +114,16 @@ def test_states_of_torchs_adamw_go_on(dtype, bits):
         # smallest fp16, so that it divides by zero.  They stay, and the step adds none.
         fine = torch.isfinite(p)
         assert bool(torch.isfinite(v).all()) and torch.equal(torch.isfinite(q), fine) and not torch.equal(p[fine], q[fine])
+
+
+def test_two_optimizers_count_their_own_captured_steps():
+    p = torch.ones(100, device=DEV, requires_grad=True)
+    p.grad = torch.ones(100, device=DEV)
+    opt = FusedAdamW([p], capturable=True)
+    opt.step()
+    q = p.detach().clone().requires_grad_(True)
+    q.grad = p.grad.clone()
+    other = FusedAdamW([q], capturable=True)
+    other.load_state_dict(opt.state_dict())
+    opt.step(), other.step(), other.step(), opt.step()
+    assert float(opt.state[p]["step"]) == float(other.state[q]["step"]) == 3 and torch.equal(p, q)
