@@ -54,6 +54,7 @@ constexpr int CHUNK = 2048;
 constexpr int NORM_BYTES = 16384, SCALE_BYTES = NORM_BYTES / 2;
 constexpr int XCDS = 8;  // workgroup b of a launch runs on XCD b % 8, which has an L2 of its own
 constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;  // workgroups of one launch (256 threads each: under 2^32 work items)
+constexpr int64_t MAX_ELEMENTS = MAX_BLOCKS * CHUNK;  // of one tensor, compared before anything is added to them
 constexpr int64_t MAX_TURNS = MAX_BLOCKS / 2 - 8;        // two workgroups of the scaling each, and what fills the last row
 constexpr int QBLOCK = FSGS_ADAMW_BLOCK;  // elements that share a power of two
 constexpr int NORM_GROUPS = 2048;      // workgroups of one norm launch at most: eight per CU
@@ -746,7 +747,7 @@ int fsgs_adamw_step(int n_tensors, const FsgsAdamWTensor *tensors, int n_hypers,
     if (on_device) regions.add(h.step_dev, 4, true);  // each tensor counts its own steps
     if (x.n == 0) continue;
     if (!x.param || !x.grad || !x.exp_avg || !x.exp_avg_sq || (state_bits == 8 && !x.scales)) return FSGS_ERR_INVALID;
-    if (chunks_of(x.n) > MAX_BLOCKS) return FSGS_ERR_INVALID;
+    if (x.n > MAX_ELEMENTS) return FSGS_ERR_INVALID;
     if (master < 0) master = x.master != nullptr;
     if (master != (x.master != nullptr) || (master && dtype == FSGS_DTYPE_F32)) return FSGS_ERR_INVALID;
     regions.add(x.param, x.n * esize, true);
@@ -828,7 +829,7 @@ int fsgs_adamw_moments(int n_tensors, const FsgsAdamWMoments *tensors, int write
   if (!regions.items) return FSGS_ERR_CAPACITY;
   for (int i = 0; i < n_tensors; i++) {
     const FsgsAdamWMoments &x = tensors[i];
-    if (x.n < 0 || chunks_of(x.n) > MAX_BLOCKS) return FSGS_ERR_INVALID;
+    if (x.n < 0 || x.n > MAX_ELEMENTS) return FSGS_ERR_INVALID;
     if (x.n == 0) continue;
     if (!x.exp_avg_q || !x.exp_avg_sq_q || !x.scales || !x.exp_avg || !x.exp_avg_sq) return FSGS_ERR_INVALID;
     regions.add(x.exp_avg_q, x.n, write != 0);

@@ -224,3 +224,23 @@ def test_a_loaded_state_shares_nothing_with_the_other_optimizer(capturable):
     assert float(st["step"]) == 4.0 and all(st[k].data_ptr() != v.data_ptr() for k, v in opt.state[p].items())
     opt.state[p]["step"].add_(1.0)
     assert float(st["step"]) == 4.0
+
+
+@pytest.mark.parametrize("n", [2 ** 63 - 1, 2 ** 63 - 2047, 2 ** 62, 2 ** 35])
+def test_sizes_past_what_a_launch_takes_are_refused(n):
+    """before anything is launched; the rounding up to whole workgroups passes 2^63 for the first"""
+    from array import array
+
+    from fsgs_amd import _lib
+
+    lib, at = _lib.load(), [(k + 1) << 40 for k in range(6)]
+    hyper = (_lib.FsgsAdamWHyper * 1)(_lib.FsgsAdamWHyper(1e-3, 0.9, 0.999, 1e-8, 0.0, 1, None, None))
+    for bits in (32, 8):
+        row = array("q", (*at[:5], 0, n, 0))
+        assert lib.fsgs_adamw_step(1, row.tobytes(), 1, hyper, 0, bits, 0, None, 0.0, None, None, 0, None, None) == _lib.FSGS_ERR_INVALID
+    for write in (0, 1):
+        assert lib.fsgs_adamw_moments(1, array("q", (*at[:5], n)).tobytes(), write, 0, None) == _lib.FSGS_ERR_INVALID
+    grads = array("q", (at[0], n, 0)).tobytes()
+    if n * 4 > 2 ** 40:
+        assert lib.fsgs_grad_norm(1, grads, 1.0, at[1], 1 << 20, at[2], at[3], None) == _lib.FSGS_ERR_INVALID
+        assert lib.fsgs_grad_scale(1, grads, at[1], None) == _lib.FSGS_ERR_INVALID
