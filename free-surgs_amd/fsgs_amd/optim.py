@@ -296,10 +296,14 @@ class FusedAdamW(torch.optim.Optimizer):
     def _blocks(p):
         return -(-p.numel() // _lib.ADAMW_BLOCK)
 
-    def _ready(self, p, st, group):
-        """the entries that the group's options ask for: made on the first step, converted where the options changed"""
+    @staticmethod
+    def _no_capture(p):
         if p.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("FusedAdamW: a parameter's state would be made inside a graph capture; run one eager step first")
+
+    def _ready(self, p, st, group):
+        """the entries that the group's options ask for: made on the first step, converted where the options changed"""
+        self._no_capture(p)
         like = dict(memory_format=torch.preserve_format)
         if group["state_bits"] == 32 and "exp_avg" not in st:
             if "exp_avg_q" in st:
@@ -423,6 +427,9 @@ class FusedAdamW(torch.optim.Optimizer):
         if m.shape != p.shape or v.shape != p.shape:
             raise ValueError("set_moments: moments of shape %s and %s for a parameter of shape %s" % (
                 tuple(m.shape), tuple(v.shape), tuple(p.shape)))
+        if not (0 <= float(step) < 2 ** 53 and float(step) == int(step)):
+            raise ValueError("set_moments: a count of steps is a whole number that is not negative, got %r" % (step,))
+        self._no_capture(p)
         st = {"step": step}
         if group["state_bits"] == 8:
             self._write(p, st, m, v)

@@ -244,3 +244,15 @@ def test_sizes_past_what_a_launch_takes_are_refused(n):
     if n * 4 > 2 ** 40:
         assert lib.fsgs_grad_norm(1, grads, 1.0, at[1], 1 << 20, at[2], at[3], None) == _lib.FSGS_ERR_INVALID
         assert lib.fsgs_grad_scale(1, grads, at[1], None) == _lib.FSGS_ERR_INVALID
+
+
+@pytest.mark.parametrize("step", [-1, 2.5, float("nan"), float("inf"), torch.tensor(-4.0)])
+def test_set_moments_refuses_counts_that_are_none(step):
+    p = torch.ones(3, requires_grad=True)
+    opt = FusedAdamW([p])
+    opt.state[p] = before = adam_state(p)
+    with pytest.raises(ValueError, match="count"):
+        opt.set_moments(p, torch.zeros(3), torch.zeros(3), step)
+    assert opt.state[p] is before and before["step"] == 3
+    opt.set_moments(p, torch.zeros(3), torch.zeros(3), torch.tensor(7.0))
+    assert opt.state[p]["step"] == 7 and type(opt.state[p]["step"]) is int

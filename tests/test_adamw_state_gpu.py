@@ -127,3 +127,20 @@ def test_two_optimizers_count_their_own_captured_steps():
     other.load_state_dict(opt.state_dict())
     opt.step(), other.step(), other.step(), opt.step()
     assert float(opt.state[p]["step"]) == float(other.state[q]["step"]) == 3 and torch.equal(p, q)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_set_moments_inside_a_capture_is_refused_and_changes_nothing(bits):
+    p = torch.ones(100, device=DEV, requires_grad=True)
+    p.grad = torch.ones(100, device=DEV)
+    opt = FusedAdamW([p], state_bits=bits, capturable=True)
+    opt.step()
+    st, before = opt.state[p], opt.moments()[0]
+    zero = torch.zeros(100, device=DEV)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.set_moments(p, zero, zero, 5)
+    torch.cuda.synchronize()
+    assert opt.state[p] is st and float(st["step"]) == 1
+    assert all(torch.equal(a, b) for a, b in zip(opt.moments()[0], before))
