@@ -486,14 +486,15 @@ class FusedAdamW(torch.optim.Optimizer):
         # (factor, bound, norm, scratch, its bytes): nothing, the bound that a single bucket applies by itself, or the factor
         # from the norm over several
         limit = (None, 0.0, None, None, 0)
-        if self.max_grad_norm is not None and len(work) == 1:
+        max_norm = None if self.max_grad_norm is None else _max_norm(self.max_grad_norm)  # it may have been set since
+        if max_norm is not None and len(work) == 1:
             nbytes = _scratch_bytes(len(work[0].params))
             norm, hold = _lib.host().norm_buffers(work[0].device.index, nbytes)
-            limit, self.last_grad_norm = (None, self.max_grad_norm, norm.data_ptr(), hold.data_ptr(), nbytes), norm
-        elif self.max_grad_norm is not None:
+            limit, self.last_grad_norm = (None, max_norm, norm.data_ptr(), hold.data_ptr(), nbytes), norm
+        elif max_norm is not None:
             found = hold = _grads_of([p for b in work for p in b.params], "FusedAdamW(max_grad_norm)")
             with _on(found.device):
-                _lib.check(found.launch(lib.fsgs_grad_norm, self.max_grad_norm), "fsgs_grad_norm")
+                _lib.check(found.launch(lib.fsgs_grad_norm, max_norm), "fsgs_grad_norm")
             limit, self.last_grad_norm = (found.factor, 0.0, None, None, 0), found.norm
         for b in work:
             n = len(b.params)

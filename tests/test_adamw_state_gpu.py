@@ -144,3 +144,22 @@ def test_set_moments_inside_a_capture_is_refused_and_changes_nothing(bits):
     torch.cuda.synchronize()
     assert opt.state[p] is st and float(st["step"]) == 1
     assert all(torch.equal(a, b) for a, b in zip(opt.moments()[0], before))
+
+
+@pytest.mark.parametrize("types", [(torch.float32,), (torch.float32, torch.bfloat16)])
+def test_a_bound_that_is_set_later_is_checked(types):
+    """with one launch sequence and with several"""
+    ps = [torch.ones(10, device=DEV, dtype=t, requires_grad=True) for t in types]
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt = FusedAdamW(ps)
+    opt.step()
+    for bad in (-1.0, float("nan")):
+        opt.max_grad_norm = bad
+        before = [p.detach().clone() for p in ps]
+        with pytest.raises(ValueError, match="max_norm"):
+            opt.step()
+        assert all(torch.equal(p, q) and opt.state[p]["step"] == 1 for p, q in zip(ps, before))
+    opt.max_grad_norm = 1
+    opt.step()
+    assert abs(float(opt.last_grad_norm) - math.sqrt(10 * len(ps))) < 1e-5
