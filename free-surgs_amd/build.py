@@ -107,10 +107,10 @@ def build_host():
     root = os.path.dirname(torch.__file__)
     inc = os.path.join(root, "include")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DNDEBUG",
-           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I" + inc,
+           '-DFSGS_TORCH_VERSION="%s"' % torch.__version__, "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I" + inc,
            "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + sysconfig.get_paths()["include"], HOST_SRC,
            "-o", HOST_LIB, "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_hip", "-ltorch_cpu", "-lc10"]
-    stamp, want = HOST_LIB.replace(".so", ".o.flags"), " ".join(cmd) + " " + torch.__version__
+    stamp, want = HOST_LIB.replace(".so", ".o.flags"), " ".join(cmd)
     same = os.path.exists(stamp) and open(stamp).read() == want
     if not same or _stale(HOST_LIB, [HOST_SRC, os.path.join(HERE, "..", "include", "fsgs.h")]):
         r = subprocess.run(cmd, capture_output=True, text=True)

@@ -359,5 +359,10 @@ PyMODINIT_FUNC PyInit__fsgs_host(void) {
       {&k_masters, "master_weights"}, {&k_maximize, "maximize"}, {&k_capturable, "capturable"}};
   for (auto &k : keys)
     if (!(*k.key = PyUnicode_InternFromString(k.name))) return nullptr;
-  return PyModule_Create(&module);
+  PyObject *m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", FSGS_TORCH_VERSION)) {  // _lib.host() compares it
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
 }

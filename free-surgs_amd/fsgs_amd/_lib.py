@@ -256,13 +256,17 @@ def host():
         path = os.path.join(_HERE, "lib", "_fsgs_host.so")
         if not os.path.exists(path):
             raise ImportError("_fsgs_host.so is missing (%s). Build it with `python free-surgs_amd/build.py`." % path)
-        import torch  # noqa: F401  (its libraries are what the extension links to)
+        import torch  # its libraries are what the extension links to
 
         with _lock:
             if _host is None:
                 loader = machinery.ExtensionFileLoader("_fsgs_host", path)
                 mod = util.module_from_spec(util.spec_from_file_location("_fsgs_host", path, loader=loader))
                 loader.exec_module(mod)
+                built = getattr(mod, "torch_version", None)
+                if built != str(torch.__version__):  # it reads torch's own structures
+                    raise ImportError("_fsgs_host.so was built for torch %s, this is torch %s. Build it again with "
+                                      "`python free-surgs_amd/build.py`." % (built, torch.__version__))
                 _host = mod
     return _host
 

@@ -256,3 +256,16 @@ def test_set_moments_refuses_counts_that_are_none(step):
     assert opt.state[p] is before and before["step"] == 3
     opt.set_moments(p, torch.zeros(3), torch.zeros(3), torch.tensor(7.0))
     assert opt.state[p]["step"] == 7 and type(opt.state[p]["step"]) is int
+
+
+def test_the_host_extension_is_loaded_for_its_own_torch_alone(monkeypatch):
+    from fsgs_amd import _lib
+
+    assert _lib.host().torch_version == torch.__version__
+    monkeypatch.setattr(_lib, "_host", None)
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    for _ in range(2):
+        with pytest.raises(ImportError, match="built for torch"):
+            _lib.host()
+    monkeypatch.undo()
+    assert _lib.host().grad_rows([], 16)[1] == -1
