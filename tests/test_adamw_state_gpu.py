@@ -163,3 +163,30 @@ def test_a_bound_that_is_set_later_is_checked(types):
     opt.max_grad_norm = 1
     opt.step()
     assert abs(float(opt.last_grad_norm) - math.sqrt(10 * len(ps))) < 1e-5
+
+
+@pytest.mark.parametrize("stepped_before", [False, True])
+def test_codes_to_values_and_back_change_no_value(stepped_before):
+    """what a densification and a checkpoint of an 8-bit run rely on.  A code is four bits times a power of two, its square eight
+    bits: the values, and the root of v, are exact in fp32, and a value that is a code's is rounded to itself."""
+    ps, gs = make([1, 7, 128, 129, 4096, 5001, 70003], torch.float32, seed=5)
+    opt = FusedAdamW(ps, state_bits=8)
+    gen = torch.Generator().manual_seed(1)
+    for p, g in zip(ps, gs):
+        n = p.numel()
+        opt.set_moments(p, (torch.randn(n, generator=gen) * torch.exp(3 * torch.randn(n, generator=gen))).to(DEV),
+                        (torch.exp(4 * torch.randn(n, generator=gen)) * (torch.rand(n, generator=gen) < 0.9)).to(DEV), 7)
+        p.grad = g
+    for _ in range(3 if stepped_before else 0):
+        opt.step()
+    before = opt.moments()
+    for p, (m, v) in zip(ps, before):
+        opt.set_moments(p, m, v, 7)
+    for _ in range(2):  # the same again, by widening
+        for p, (m, v), (m2, v2) in zip(ps, before, opt.moments()):
+            assert torch.equal(m, m2) and torch.equal(v, v2) and bool(m.any()) and bool(v.any())
+            opt.widen(p)
+            st = opt.state[p]
+            assert torch.equal(st["exp_avg"], m) and torch.equal(st["exp_avg_sq"], v)
+            opt._ready(p, st, opt.param_groups[0])
+            assert "exp_avg_q" in st and "exp_avg" not in st
