@@ -19,9 +19,9 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
     "-ffp-contract=on", "-Wno-unused-result", "-DNDEBUG",
-    # no SLP vectoriser: where two FMAs belong in one v_pk_fma_f32 the kernels say so (float2v); the pairs the vectoriser
-    # forms on its own need register shuffles -- and, in streaming loops, copies of loads still in flight -- that cost
-    # blend_bwd 5 % and exposed a memory round trip per row in photometric_bwd (DESIGN s3, round 3)
+    # no SLP vectoriser: the pairs that it forms need register shuffles -- and, in streaming loops, copies of loads still in
+    # flight -- that cost blend_bwd 5 % and exposed a memory round trip per row in photometric_bwd (measured where packed fp32
+    # instructions were still in use)
     "-fno-slp-vectorize",
     # no packed fp32 instructions: some of their forms have given wrong results now and then on this hardware, in ways a
     # test does not reliably show.  A float2v fma becomes two plain ones with the same rounding; a 1280x1024 / 300 000-Gaussian

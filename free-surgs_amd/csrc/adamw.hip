@@ -7,7 +7,8 @@
 // A few dozen operations an element against 16 to 30 bytes: everything here is bound by HBM, so each kernel reads and writes
 // every array once, with 16-byte accesses where the type allows, and one launch takes up to 48 tensors (192 gradients).
 // The step's loads and stores are non-temporal, what they move is next used a whole step later: 1 M Gaussians (59 M floats)
-// 311 -> 280 us (5.9 TB/s) with 32-bit moments, 176 -> 155 us (6.1 TB/s) with 8-bit ones; on the loads or on the stores
+// 311 -> 280 us (5.9 TB/s) with 32-bit moments, 176 -> 155 us (6.1 TB/s) with 8-bit ones (both sides in one run; 150 to 160
+// us over runs and cards); on the loads or on the stores
 // alone there is next to nothing to gain (302 and 313 us).  The norm's and the scaling's are not: gradients come from a
 // cache as often as not (20 M bf16: 15.6 us against 17.7).
 //
@@ -49,8 +50,9 @@ constexpr int THREADS = 256;
 // Elements of one workgroup of a step: two vectors a thread and array.  Four make fewer, larger workgroups (20 k Gaussians,
 // 1.2 M floats: 10.1 us against 8.1; 24 bf16 layers of 20 M in 8 bits: 59 us against 54; no difference at 59 M).
 constexpr int CHUNK = 2048;
-// Bytes of one workgroup's turn in the norm, four 16-byte vectors a thread; the scaling's workgroups take half of one (160 bf16
-// layers of 64 M: norm 27.6 us, with two vectors 30.9, with eight 28.5; scaling 48.0 us, with four 51.7, with one 60.1).
+// Bytes of one workgroup's turn in the norm, four 16-byte vectors a thread; the scaling's workgroups take half of one.  Inside a
+// clip, two / four / eight vectors: 160 bf16 layers of 64 M: norm 33.6 / 34.2 / 36.3 us; 17.7 M floats 13.6 / 13.0 / 12.6.
+// Scaling with one / two / four: 40.8 / 37.2 / 37.6 and 20.7 / 20.9 / 20.3.
 constexpr int NORM_BYTES = 16384, SCALE_BYTES = NORM_BYTES / 2;
 constexpr int XCDS = 8;  // workgroup b of a launch runs on XCD b % 8, which has an L2 of its own
 constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;  // workgroups of one launch (256 threads each: under 2^32 work items)
@@ -99,8 +101,7 @@ template <int WAVES> __device__ __forceinline__ double group_sum(double a, doubl
 // The factor on the gradients: one that another launch has left, or formed here from up to SUMMED partial sums of the squares.
 // A launch costs the host 4 us and the GPU 2 to 3; a small step's or scaling's workgroups rather add the sums themselves, one a
 // thread, 2 KB from the cache each: clipping 40 tensors of 0.3 M floats 17.6 -> 14.5 us, and at the border (1 M floats, 245
-// sums) 12.2 us against 13.9 back to back.  More sums than threads are left to the launch: the workgroups that would add
-// them grow in number with them, and the host's time is no longer what counts.
+// sums) 12.2 us against 13.9 back to back.  More sums than threads are left to the launch; other borders have not been measured.
 struct Bound {
   const double *partial;
   const float *factor;
@@ -325,8 +326,8 @@ __device__ __forceinline__ void adamw8_one(float &w, float g, float &m, float &r
   w = fmaf(w, h.decay, -h.step_size * (m / fmaf(r, h.inv_bc2_sqrt, h.eps)));
 }
 
-// 16.03 bytes an element in fp32: 1 M Gaussians 157 us = 6.0 TB/s (354 MB written, 590 MB read), 24 bf16 tensors of 20 M with
-// masters 53 us.  It runs 88 vector instructions an element, half of what the SIMDs could issue in that time: approximate roots
+// 16.03 bytes an element in fp32: 1 M Gaussians 157 us = 6.0 TB/s (354 MB written, 590 MB read; 150 to 160 us over runs and
+// cards), 24 bf16 tensors of 20 M with masters 54 us.  It runs 88 vector instructions an element, half of what the SIMDs could issue in that time: approximate roots
 // and quotients (a fifth fewer) change nothing, so the exact ones stay.  The codes' four-byte accesses are plain: made
 // non-temporal they cost 5 % (165 us), the 64 bytes of a half block being too little for a line.
 template <typename T, bool MASTER> __global__ __launch_bounds__(THREADS) void adamw8_kernel(Table t) {
@@ -415,7 +416,7 @@ struct MomentTable {
 };
 static_assert(sizeof(MomentTable) <= 4096, "kernel argument");
 
-// 2 bytes in and 4 out for bf16: 1 M Gaussians 60 us = 5.8 TB/s.
+// 2 bytes in and 4 out for bf16: 1 M Gaussians 57 us = 6.2 TB/s.
 // v = r^2 of a four-bit code has eight significant bits: bf16 holds m and v exactly (within its range)
 template <typename T> __global__ __launch_bounds__(THREADS) void moments_read_kernel(MomentTable t) {
   const int k = owner<TENSORS>(t.start, t.count, blockIdx.x);
@@ -579,8 +580,8 @@ struct Squares {
 };
 
 // Squares are summed in 64 bits (no overflow, no loss over long sums), each workgroup over its own turns in a fixed order:
-// the same gradients give the same norm to the last bit.  17.7 M floats 11 us, 64 M bf16 in 160 tensors 24 us = 5.4 TB/s, and
-// 2 to 4 us for the second launch, which adds up to 2048 partial sums (1024 workgroups are slower at 64 M, 4096 at 17.7 M).
+// the same gradients give the same norm to the last bit.  17.7 M floats 13 us, 64 M bf16 in 160 tensors 34 us behind a scaling
+// whose lines are still being written back, and 2 to 5 us for the second launch, which adds up to 2048 partial sums (1024 workgroups are slower at 64 M, 4096 at 17.7 M).
 // Held to 64 registers (eight waves a SIMD): the compiler's own choice, 128, takes 10 % longer.
 __global__ __launch_bounds__(THREADS, 8) void norm_partial_kernel(GradTable t, double *partial) {
   __shared__ double lds[THREADS / 64];
@@ -603,8 +604,8 @@ __global__ __launch_bounds__(1024) void norm_finish_kernel(const double *partial
 }
 
 // The turns that the norm read last come first, each on the XCD that read it, whose L2 may still hold it: clipping 5.9 M floats
-// 20.0 -> 16.5 us, 17.7 M 37.3 -> 35.6 (the scaling 21 us, 6.7 TB/s), 20 M bf16 25.2 -> 23.4, 64 M bf16 73 -> 71, 59 M floats
-// as before; in the reverse order on any XCD, or on the same XCD in the norm's order, only the smallest gains.
+// 20.0 -> 16.5 us, 17.7 M 37.3 -> 35.6 (the scaling 21 us, 6.7 TB/s), 20 M bf16 25.2 -> 23.4, 64 M bf16 77 -> 75 (on another
+// card 73 -> 71), 59 M floats as before; in the reverse order on any XCD, or on the same XCD in the norm's order, only the smallest gains.
 // Non-temporal loads and stores would make it faster by itself where the gradients outgrow the 256 MB cache (norm and scaling of
 // 59 M floats 134 -> 111 us), but the step that follows then reads them from HBM: both together 380 -> 394 us, 111 -> 115 at
 // 17.7 M.

@@ -180,7 +180,8 @@ def grad_norm(tensors):
 
 
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
-    """torch.nn.utils.clip_grad_norm_ in three launches per 192 tensors: the gradients' global 2-norm, and every gradient
+    """torch.nn.utils.clip_grad_norm_ in two launches for every 192 tensors (norm, scaling), and one between them where all
+    gradients make more than 256 pieces of 16 KB: the gradients' global 2-norm, and every gradient
     (dense, on one device, float32 / bfloat16 / float16 side by side) scaled in place by min(1, max_norm / (norm + 1e-6));
     where that factor is 1 no gradient is read again.  Returns the norm (0-d float32) without a host synchronisation, unless
     error_if_nonfinite asks for one."""
