@@ -428,9 +428,9 @@ class FusedAdamW(torch.optim.Optimizer):
         if m.shape != p.shape or v.shape != p.shape:
             raise ValueError("set_moments: moments of shape %s and %s for a parameter of shape %s" % (
                 tuple(m.shape), tuple(v.shape), tuple(p.shape)))
+        self._no_capture(p)
         if not (0 <= float(step) < 2 ** 53 and float(step) == int(step)):
             raise ValueError("set_moments: a count of steps is a whole number that is not negative, got %r" % (step,))
-        self._no_capture(p)
         st = {"step": step}
         if group["state_bits"] == 8:
             self._write(p, st, m, v)
